@@ -289,6 +289,82 @@ void yan_b200_set_wait_timeout_ns(unsigned long long timeout_ns);
  * comm/gemm_allreduce.cu:403-410). */
 void yan_b200_set_collective_timeout_ns(unsigned long long timeout_ns);
 
+/* ---- training a layer ---------------------------------------------------------------------------------------------------------
+ * No counterpart in the reference.  Element types of the arguments below: */
+enum { YAN_B200_F32 = 0, YAN_B200_BF16 = 1 };
+
+/*
+ * Weight gradient of a linear layer, out[n, k] (+)= sum over m of dy[m, n] * x[m, k], from operands quantized to e4m3 with one power of
+ * two per feature and block of 128 tokens (the smallest 2^e with amax <= 448 * 2^e, e >= -127), summed in fp32.
+ * dy [m, n], x [m, k]: bf16, rows dy_ld and x_ld elements apart, any alignment (rows that start on 32-byte boundaries with a multiple of
+ * 16 columns are the fast case); out [n, out_ld] fp32 or bf16, rounded once.  accumulate != 0: added to what out holds.  m = 0 is a sum
+ * of nothing.  What is not finite in a column of dy (x) makes that row (column) of out NaN.
+ * workspace: yan_b200_fp8_linear_wgrad_workspace_bytes(m, n, k, 0, num_sms) bytes on a 256-byte boundary for the codes, scales and
+ * partial tiles; its content does not matter.  Calls that may overlap need one each.
+ */
+size_t yan_b200_fp8_linear_wgrad_workspace_bytes(int m, int n, int k, int num_groups, int num_sms);
+void yan_b200_fp8_linear_wgrad(const void* dy, const void* x, void* out, int m, int n, int k, long long dy_ld, long long x_ld,
+                               long long out_ld, int out_dtype, int accumulate, void* workspace, size_t workspace_bytes,
+                               void* stream, int num_sms, int* return_code);
+
+/*
+ * The same for every group of rows (expert) its own: out[g] over rows [group_starts[g], group_starts[g] + group_sizes[g]) of dy and x,
+ * blocks of 128 counted from the first row of the group.  Both lists are int32 on the device; starts need no alignment, rows outside of
+ * every group are not read, groups do not overlap.  A list that reaches outside of [0, m) is cut to it.  num_groups <= 512.
+ * A group without rows gives zeros (nothing is added with accumulate).
+ * out [num_groups, n, out_ld], out_group_stride elements from one group to the next.
+ */
+void yan_b200_k_grouped_fp8_linear_wgrad(const void* dy, const void* x, void* out, const int* group_starts, const int* group_sizes,
+                                         int num_groups, int m, int n, int k, long long dy_ld, long long x_ld, long long out_ld,
+                                         long long out_group_stride, int out_dtype, int accumulate, void* workspace,
+                                         size_t workspace_bytes, void* stream, int num_sms, int* return_code);
+
+/*
+ * One AdamW step over num_tensors tensors (any number; a launch takes 420 of them).  Per element, in fp32, with t = step >= 1:
+ *   g = grad * *grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ * param_dtype and grad_dtype: YAN_B200_F32 or YAN_B200_BF16, the same for all tensors.  state_bits 32: exp_avg and exp_avg_sq hold m
+ * and v in fp32.  state_bits 8: they hold e4m3 codes of m and of sqrt(v), and the scale arrays one power of two for each 128 elements,
+ * ceil(numel / 128) floats: m = code * scale.  A new state is all zeros in either case.
+ * grad_scale: optional fp32 on the device (gradient clipping, loss scaling).  copy: optional, receives the new parameters in bf16.
+ * Pointers need the alignment of their type; where all of a tensor's allow four elements at a time (16 bytes in fp32, 8 in bf16, 4 for
+ * codes) it is read and written that way.  The list itself is on the host and may go when the call returns.
+ */
+typedef struct {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    void* copy;
+    long long numel;
+    double weight_decay;
+} yan_b200_adamw_tensor;
+
+void yan_b200_adamw_step(const yan_b200_adamw_tensor* tensors, int num_tensors, int param_dtype, int grad_dtype, int state_bits,
+                         double lr, double beta1, double beta2, double eps, long long step, const float* grad_scale, void* stream,
+                         int* return_code);
+
+/*
+ * Balance loss of a router, the selections per expert, and the gradient of the loss.  For the tokens of sequence s that count, n_s of
+ * them, with p[t] = softmax(logits[t]) or sigmoid(logits[t]) / sum of sigmoid(logits[t]):
+ *   counts[s, e] = selections of e among them;  P[s, e] = sum of p[t, e];  loss = coef / sequences * sum over s of
+ *   experts / (top n_s^2) * sum over e of counts[s, e] * P[s, e];  grad = d loss / d logits, the counts being constants.
+ * logits [tokens, experts] fp32 or bf16, rows logits_ld elements apart; expert_ids [tokens, top] int32 or int64 (ids_64), contiguous; an
+ * id outside of [0, experts) is no selection.  token_mask: optional, a byte per token, 0 = does not count (its logits are not read).
+ * cu_seqlens: optional int32 [sequences + 1] on the device, ascending; without it sequences = 1.  Tokens outside of every sequence do
+ * not count; a sequence without tokens adds nothing.  loss: one fp32; counts int32 [sequences, experts]; grad: optional, of the
+ * logits' type, zero for tokens that do not count.  experts <= 1024.
+ * workspace: yan_b200_moe_balance_loss_workspace_bytes(...) bytes on a 256-byte boundary; its content does not matter.
+ */
+enum { YAN_B200_SOFTMAX = 0, YAN_B200_SIGMOID = 1 };
+size_t yan_b200_moe_balance_loss_workspace_bytes(int tokens, int experts, int sequences, int with_grad, int num_sms);
+void yan_b200_moe_balance_loss(const void* logits, const void* expert_ids, const void* token_mask, const int* cu_seqlens, float* loss,
+                               int* counts, void* grad, int tokens, int experts, int top, int sequences, long long logits_ld,
+                               long long grad_ld, int logits_dtype, int ids_64, int score, float coef, void* workspace,
+                               size_t workspace_bytes, void* stream, int num_sms, int* return_code);
+
 #ifdef __cplusplus
 }
 #endif

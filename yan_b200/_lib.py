@@ -20,6 +20,9 @@ LIB_PATH = os.environ.get("YAN_B200_LIBRARY") or os.path.join(_PKG_DIR, "lib", "
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_longlong
+_Z = ctypes.c_size_t
+_D = ctypes.c_double
 _RC = ctypes.POINTER(ctypes.c_int)
 
 # name -> (restype, argtypes); mirrors include/yan_b200.h one to one.
@@ -50,6 +53,13 @@ SIGNATURES = {
     "yan_b200_fp8_linear_workspace_bytes": (ctypes.c_size_t, [_I, _I]),
     "yan_b200_fp8_linear_bf16": (None, [_P, _P, _P, _P, _P, ctypes.c_size_t, _I, _I, _I, _I, _P, _I, _I, _RC]),
     "yan_b200_fp8_linear_bf16_static": (None, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _RC]),
+    "yan_b200_fp8_linear_wgrad_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "yan_b200_fp8_linear_wgrad": (None, [_P, _P, _P, _I, _I, _I, _L, _L, _L, _I, _I, _P, _Z, _P, _I, _RC]),
+    "yan_b200_k_grouped_fp8_linear_wgrad": (None, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _I, _I, _P, _Z, _P, _I, _RC]),
+    "yan_b200_adamw_step": (None, [_P, _I, _I, _I, _I, _D, _D, _D, _D, _L, _P, _P, _RC]),
+    "yan_b200_moe_balance_loss_workspace_bytes": (_Z, [_I, _I, _I, _I, _I]),
+    "yan_b200_moe_balance_loss": (None, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _I, _I, _I, ctypes.c_float, _P, _Z, _P, _I,
+                                         _RC]),
     "yan_b200_read_device_status": (None, [_RC, _I, _RC]),
     "yan_b200_wait_probe": (None, [ctypes.c_ulonglong, _P, _RC]),
     "yan_b200_set_programmatic_dependent_launch": (None, [_I]),
@@ -62,6 +72,13 @@ SIGNATURES = {
 STATIC_SCRATCH_MAX_ELEMENTS = 8 << 20
 
 FASTCALL_PATH = os.path.join(_PKG_DIR, "lib", "_fastcall.so")
+
+
+class AdamwTensor(ctypes.Structure):
+    """yan_b200_adamw_tensor of include/yan_b200.h."""
+    _fields_ = [("param", _P), ("grad", _P), ("exp_avg", _P), ("exp_avg_sq", _P), ("exp_avg_scale", _P), ("exp_avg_sq_scale", _P),
+                ("copy", _P), ("numel", _L), ("weight_decay", _D)]
+
 
 _lib: Optional[ctypes.CDLL] = None
 _fast = None

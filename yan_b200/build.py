@@ -121,7 +121,7 @@ def _build_cuda_library(force: bool, verbose: bool) -> str:
         obj = os.path.join(OBJ_DIR, f"gemm_inst_bn{bn}.o")
         jobs.append(([nvcc, *NVCC_FLAGS, *extra, f"-DYAN_BLOCK_N={bn}", f"-I{INCLUDE_DIR}", "-c",
                       os.path.join(CSRC_DIR, "gemm_inst.cu"), "-o", obj], obj))
-    for name in ("capi",):
+    for name in ("capi", "train"):
         obj = os.path.join(OBJ_DIR, f"{name}.o")
         jobs.append(([nvcc, *NVCC_FLAGS, *extra, f"-I{INCLUDE_DIR}", "-c", os.path.join(CSRC_DIR, f"{name}.cu"),
                       "-o", obj], obj))

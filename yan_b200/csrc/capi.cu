@@ -10,6 +10,7 @@
 #include "../../include/yan_b200.h"
 #include "gemm_dispatch.h"
 #include "launch_order.h"
+#include "launch_state.h"
 #include "gemm/fp8_gemm_masked_few_rows.cuh"
 #include "gemm/fp8_gemm_small_m.cuh"
 #include "gemm/fp8_gemm_stacked_k.cuh"
@@ -31,6 +32,10 @@ long long* g_clock_probe = nullptr;
 constexpr int kMaxDevices = 64;
 int* g_status_ptr[kMaxDevices] = {};
 
+}  // namespace
+
+namespace yan {
+
 int* status_word_of_current_device() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
@@ -44,6 +49,14 @@ int* status_word_of_current_device() {
     }
     return g_status_ptr[dev];
 }
+
+unsigned long long wait_timeout_ns() { return g_timeout_ns; }
+
+}  // namespace yan
+
+namespace {
+
+using yan::status_word_of_current_device;
 
 // Scratch of the allocation-free entry point: quantized activations followed by their scales.
 // Every device that loads this library holds these bytes until the process exits.

@@ -66,9 +66,10 @@ struct GemmParams {
 namespace detail {
 
 // Wait on an mbarrier phase with a wall-clock bound.  Returns false when the wait ran out or another
-// role already gave up; the caller then leaves its loop.
+// role already gave up; the caller then leaves its loop.  Params: what holds a launch's `status` and `timeout_ns`.
+template <typename Params>
 __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag,
-                                             const GemmParams& p, int site) {
+                                             const Params& p, int site) {
     if (ptx::mbar_try_wait(bar, parity)) return true;
     // Fast path first: when the phase is already complete (the usual case for the role that bounds the kernel) the
     // timer is never read.

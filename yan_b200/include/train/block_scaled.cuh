@@ -1,0 +1,77 @@
+#pragma once
+// tcgen05 products of e4m3 operands whose scales the tensor core applies (kind::mxf8f6f4): one power of two (UE8M0, a byte that
+// stands for 2^(byte - 127)) per row and 32 values of the summed dimension.  Here a scale holds for 128 values, so the four
+// instructions of a 128-wide k-block name the same byte.
+//
+// Operands are M- (N-) major: a k-block of a [tokens, features] matrix is 128 rows (tokens, the summed dimension) of 128 bytes
+// (features) in shared memory, as TMA writes them with the 128-byte swizzle, and the tensor core transposes on its way.
+//
+// Scales in tensor memory: the byte of row r is in lane r % 32 (and again in lanes 32.., 64.., 96..), column r / 32, and the four bytes of
+// that 32-bit cell belong to four successive k-blocks.  `scale_tile` is that cell block of 128 rows and four k-blocks as 512 bytes in
+// memory, [row % 32][row / 32][k-block % 4], which tcgen05.cp.32x128b.warpx4 copies as it stands.
+
+#include <cstdint>
+
+#include "../gemm/mma_utils.cuh"
+#include "../gemm/ptx.cuh"
+
+namespace yan {
+
+constexpr uint32_t kScaleTileBytes = 512;  // 128 rows x 4 k-blocks
+
+// Byte of (row, k-block) in its scale tile; row < 128, kb < 4.
+__host__ __device__ constexpr uint32_t scale_tile_offset(uint32_t row, uint32_t kb) { return (row % 32) * 16 + (row / 32) * 4 + kb; }
+
+// --- instruction descriptor for kind::mxf8f6f4 ---
+//  [4,6)  which byte of a cell holds B's scale   [7,10), [10,13) formats: 0 = e4m3   [15], [16] A, B are M- / N-major
+//  [17,23) N >> 3   [23] scale format: 1 = UE8M0   [24,29) M >> 4   [29,31) which byte holds A's scale
+__host__ __device__ constexpr uint32_t make_instr_desc_mx_mn_major(uint32_t umma_m, uint32_t umma_n) {
+    return (1u << 15) | (1u << 16) | ((umma_n >> 3) << 17) | (1u << 23) | ((umma_m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t with_scale_byte(uint32_t idesc, uint32_t byte) { return idesc | (byte << 4) | (byte << 29); }
+
+// --- shared-memory descriptor of an M-major operand, 128-byte swizzle ---
+// Stride offset: from 8 rows of the summed dimension to the next 8 (1024 bytes); leading offset: from 128 features to the next 128
+// (a box of 128 x 128 bytes).
+constexpr uint32_t kMnBoxBytes = 128 * 128;
+__device__ __forceinline__ uint64_t make_smem_desc_mn_major_sw128(uint32_t smem_addr) {
+    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kMnBoxBytes >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+// 32 values of the summed dimension are 32 rows of 128 bytes.
+constexpr uint32_t kMnKStep = (kUmmaK * 128) >> 4;
+
+// --- shared-memory descriptor of a scale tile: 32 rows of 16 bytes, 8 of them (128 bytes) per core matrix, no swizzle ---
+__device__ __forceinline__ uint64_t make_smem_desc_scales(uint32_t smem_addr) {
+    return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+
+namespace ptx {
+
+// 512 bytes of scales, shared memory -> four columns of tensor memory, in all four lane quarters.  Issued by the thread that issues the
+// products; a product issued behind it sees the scales.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void umma_mxf8f6f4_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tmem_scale_a,
+                                                 uint32_t tmem_scale_b, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_scale_a), "r"(tmem_scale_b), "r"(accumulate)
+        : "memory");
+}
+
+// Untiled bulk copy; both addresses and the size are multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
+                 "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+}  // namespace ptx
+}  // namespace yan

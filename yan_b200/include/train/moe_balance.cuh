@@ -1,0 +1,403 @@
+#pragma once
+// Balance loss of a router over experts, its gradient and the selections per expert.  For the tokens t of sequence s that count, n_s of
+// them, with p[t] = softmax(z[t]) or sigmoid(z[t]) / sum sigmoid(z[t]) over E experts and k selections per token:
+//     c[s, e] = selections of e,  P[s, e] = sum over t of p[t, e],  a[s, e] = coef / S * E / (k n_s^2) * c[s, e]
+//     loss = sum over s, e of a[s, e] * P[s, e]
+//     softmax: dz_j = p_j (a_j - sum over e of a_e p_e);  sigmoid: dz_j = s_j (1 - s_j) / sum(s) * (a_j - sum over e of a_e p_e)
+// Three launches: sums over strips of tokens, the sums of the strips with a and the loss, the gradient.  No sum depends on the order
+// in which anything runs.
+//
+// A strip is a fixed range of tokens; it may touch several sequences, and the sums of (strip, sequence) go to slot strip + sequence:
+// both grow along the tokens, so that no two pairs share a slot and those of one sequence follow one another.
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "../gemm/ptx.cuh"
+#include "../gemm/utils.cuh"
+
+namespace yan {
+
+constexpr uint32_t kMaxBalanceExperts = 1024;
+constexpr uint32_t kBalanceThreads = 256, kBalanceWarps = kBalanceThreads / 32;
+
+struct BalanceParams {
+    const void* logits = nullptr;
+    uint64_t logits_ld = 0;
+    const void* ids = nullptr;            // [tokens][top], int64 or int32; what is no expert selects nothing
+    uint32_t ids_64 = 0;
+    const uint8_t* mask = nullptr;        // optional, [tokens]: 0 = does not count
+    const int* cu_seqlens = nullptr;      // optional, [sequences + 1]
+    uint32_t tokens = 0, experts = 0, top = 0, sequences = 1;
+    uint32_t sigmoid = 0;
+    float coef = 0.0f;
+    float* loss = nullptr;
+    int* counts = nullptr;                // [sequences][experts]
+    void* grad = nullptr;                 // [tokens][grad_ld], optional
+    uint64_t grad_ld = 0;
+    uint32_t strips = 0, strip_tokens = 0;
+    // scratch
+    float* slot_sums = nullptr;           // [strips + sequences][experts]
+    int* slot_counts = nullptr;           // the same
+    int* slot_tokens = nullptr;           // [strips + sequences]
+    float* weights = nullptr;             // a, [sequences][experts]
+    float* losses = nullptr;              // [sequences][ceil(experts / 32)]
+    float2* rows = nullptr;               // [tokens]: what the gradient needs of a row's softmax (largest logit, 1 / sum)
+};
+
+namespace detail {
+
+// Tokens of sequence s that exist.
+__device__ __forceinline__ void sequence_range(const BalanceParams& p, uint32_t s, uint32_t& begin, uint32_t& end) {
+    if (p.cu_seqlens == nullptr) {
+        begin = 0, end = p.tokens;
+        return;
+    }
+    const int limit = static_cast<int>(p.tokens);
+    begin = min(max(ptx::ld_global(p.cu_seqlens + s), 0), limit);
+    end = max(min(ptx::ld_global(p.cu_seqlens + s + 1), limit), static_cast<int>(begin));
+}
+
+// First sequence that ends behind `token` (sequences if there is none); ends do not decrease.
+__device__ __forceinline__ uint32_t first_sequence_behind(const BalanceParams& p, uint32_t token) {
+    if (p.cu_seqlens == nullptr) return 0;
+    uint32_t low = 0, high = p.sequences;
+    while (low < high) {
+        const uint32_t mid = (low + high) / 2;
+        if (ptx::ld_global(p.cu_seqlens + mid + 1) > static_cast<int>(token)) high = mid;
+        else low = mid + 1;
+    }
+    return low;
+}
+
+// How the experts of a row lie over the lanes: kLanes lanes per row, kIter times kVec neighbouring experts each.
+template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
+struct BalanceRow {
+    static constexpr uint32_t kPerLane = kVec * kIter, kRowsPerWarp = 32 / kLanes;
+
+    __device__ __forceinline__ static uint32_t column(uint32_t lane, uint32_t c) {
+        return (c / kVec * kLanes + lane % kLanes) * kVec + c % kVec;
+    }
+    // A row that does not count, and experts that do not exist, read as -inf: probability zero.
+    __device__ __forceinline__ static void load(const T* row, bool there, uint32_t experts, uint32_t lane, float (&z)[kPerLane]) {
+#pragma unroll
+        for (uint32_t i = 0; i < kIter; ++i) {
+            const uint32_t col = column(lane, i * kVec);
+            if constexpr (kVec == 1) {
+                z[i] = there && col < experts ? static_cast<float>(row[col]) : -INFINITY;
+            } else {
+                uint4 v;
+                const uint32_t nothing = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+                v = make_uint4(nothing, nothing, nothing, nothing);
+                if (there && col < experts) v = *reinterpret_cast<const uint4*>(row + col);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    if constexpr (sizeof(T) == 4) {
+                        z[i * 4 + j] = __uint_as_float(w[j]);
+                    } else {
+                        z[i * 8 + 2 * j] = __uint_as_float(w[j] << 16);
+                        z[i * 8 + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ static void store(T* row, uint32_t experts, uint32_t lane, const float (&z)[kPerLane]) {
+#pragma unroll
+        for (uint32_t i = 0; i < kIter; ++i) {
+            const uint32_t col = column(lane, i * kVec);
+            if (col >= experts) continue;
+            if constexpr (kVec == 1) {
+                row[col] = static_cast<T>(z[i]);
+            } else if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float4*>(row + col) = make_float4(z[i * 4], z[i * 4 + 1], z[i * 4 + 2], z[i * 4 + 3]);
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const __nv_bfloat162 t = __floats2bfloat162_rn(z[i * 8 + 2 * j], z[i * 8 + 2 * j + 1]);
+                    w[j] = *reinterpret_cast<const uint32_t*>(&t);
+                }
+                *reinterpret_cast<uint4*>(row + col) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+    __device__ __forceinline__ static float sum(float v) {
+#pragma unroll
+        for (uint32_t off = kLanes / 2; off >= 1; off /= 2) v += __shfl_xor_sync(0xffffffffu, v, off);
+        return v;
+    }
+    __device__ __forceinline__ static float largest(float v) {
+#pragma unroll
+        for (uint32_t off = kLanes / 2; off >= 1; off /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+        return v;
+    }
+    // z -> scores that add up to 1 / inverse; `shift` is the largest logit (softmax).  A row of nothing but -inf has zeros.
+    __device__ __forceinline__ static void scores(bool sigmoid, float (&z)[kPerLane], float shift) {
+#pragma unroll
+        for (uint32_t c = 0; c < kPerLane; ++c)
+            z[c] = sigmoid ? __fdividef(1.0f, 1.0f + __expf(-z[c])) : __expf(z[c] - shift);
+    }
+};
+
+}  // namespace detail
+
+template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
+__global__ void __launch_bounds__(kBalanceThreads) balance_sums_kernel(const BalanceParams p) {
+    using Row = detail::BalanceRow<T, kVec, kLanes, kIter>;
+    constexpr uint32_t kPerLane = Row::kPerLane;
+    extern __shared__ float s_sums[];  // [warps][experts]
+    __shared__ int s_counts[kMaxBalanceExperts];
+    __shared__ int s_tokens;
+    ptx::grid_dependency_wait();
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t strip = blockIdx.x, first = strip * p.strip_tokens, last = min(first + p.strip_tokens, p.tokens);
+    const T* logits = static_cast<const T*>(p.logits);
+    for (uint32_t s = detail::first_sequence_behind(p, first); s < p.sequences; ++s) {
+        uint32_t begin, end;
+        detail::sequence_range(p, s, begin, end);
+        if (begin >= last) break;
+        begin = max(begin, first), end = min(end, last);
+        if (begin >= end) continue;
+        for (uint32_t e = threadIdx.x; e < p.experts; e += kBalanceThreads) s_counts[e] = 0;
+        if (threadIdx.x == 0) s_tokens = 0;
+        __syncthreads();
+        // selections
+        const uint64_t pairs = static_cast<uint64_t>(end - begin) * p.top;
+        for (uint64_t i = threadIdx.x; i < pairs; i += kBalanceThreads) {
+            const uint32_t token = begin + static_cast<uint32_t>(i / p.top);
+            if (p.mask != nullptr && p.mask[token] == 0) continue;
+            const uint64_t at = static_cast<uint64_t>(begin) * p.top + i;
+            const long long id = p.ids_64 != 0 ? static_cast<const long long*>(p.ids)[at] : static_cast<const int*>(p.ids)[at];
+            if (id >= 0 && id < static_cast<long long>(p.experts)) atomicAdd(&s_counts[id], 1);
+        }
+        // probabilities
+        float sums[kPerLane];
+#pragma unroll
+        for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = 0.0f;
+        int counted = 0;
+        for (uint32_t base = begin + warp * Row::kRowsPerWarp; base < end; base += kBalanceWarps * Row::kRowsPerWarp) {
+            const uint32_t token = base + lane / kLanes;
+            const bool counts = token < end && (p.mask == nullptr || p.mask[token] != 0);
+            float z[kPerLane];
+            Row::load(logits + static_cast<uint64_t>(token) * p.logits_ld, counts, p.experts, lane, z);
+            float shift = 0.0f;
+            if (p.sigmoid == 0) {
+                shift = z[0];
+#pragma unroll
+                for (uint32_t c = 1; c < kPerLane; ++c) shift = fmaxf(shift, z[c]);
+                shift = Row::largest(shift);
+                if (shift == -INFINITY) shift = 0.0f;
+            }
+            Row::scores(p.sigmoid != 0, z, shift);
+            float total = 0.0f;
+#pragma unroll
+            for (uint32_t c = 0; c < kPerLane; ++c) total += z[c];
+            total = Row::sum(total);
+            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = fmaf(z[c], inverse, sums[c]);
+            if (lane % kLanes == 0 && counts) {
+                if (p.grad != nullptr) p.rows[token] = make_float2(shift, inverse);
+                ++counted;
+            }
+        }
+        if (counted != 0) atomicAdd(&s_tokens, counted);
+#pragma unroll
+        for (uint32_t c = 0; c < kPerLane; ++c) {
+#pragma unroll
+            for (uint32_t off = kLanes; off < 32; off *= 2) sums[c] += __shfl_xor_sync(0xffffffffu, sums[c], off);
+            const uint32_t col = Row::column(lane, c);
+            if (lane < kLanes && col < p.experts) s_sums[warp * p.experts + col] = sums[c];
+        }
+        __syncthreads();
+        const uint64_t slot = strip + s;
+        for (uint32_t e = threadIdx.x; e < p.experts; e += kBalanceThreads) {
+            float sum = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kBalanceWarps; ++w) sum += s_sums[w * p.experts + e];
+            p.slot_sums[slot * p.experts + e] = sum;
+            p.slot_counts[slot * p.experts + e] = s_counts[e];
+        }
+        if (threadIdx.x == 0) p.slot_tokens[slot] = s_tokens;
+        __syncthreads();
+    }
+}
+
+// One CTA: 32 experts of one sequence; eight threads share an expert's slots.
+__global__ void __launch_bounds__(kBalanceThreads) balance_weights_kernel(const BalanceParams p) {
+    __shared__ float s_sum[8][32];
+    __shared__ int s_count[8][32], s_tokens[8];
+    ptx::grid_dependency_wait();
+    const uint32_t s = blockIdx.y, e = blockIdx.x * 32 + threadIdx.x % 32, part = threadIdx.x / 32;
+    uint32_t begin, end;
+    detail::sequence_range(p, s, begin, end);
+    float sum = 0.0f;
+    int count = 0, tokens = 0;
+    if (begin < end) {
+        const uint64_t from = begin / p.strip_tokens + s, to = (end - 1) / p.strip_tokens + s;
+        for (uint64_t slot = from + part; slot <= to; slot += 8) {
+            if (e < p.experts) {
+                sum += p.slot_sums[slot * p.experts + e];
+                count += p.slot_counts[slot * p.experts + e];
+            }
+            tokens += p.slot_tokens[slot];
+        }
+    }
+    s_sum[part][threadIdx.x % 32] = sum;
+    s_count[part][threadIdx.x % 32] = count;
+    if (threadIdx.x % 32 == 0) s_tokens[part] = tokens;
+    __syncthreads();
+    if (part != 0) return;
+    sum = 0.0f, count = 0, tokens = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) sum += s_sum[i][threadIdx.x], count += s_count[i][threadIdx.x], tokens += s_tokens[i];
+    const float n = static_cast<float>(tokens);
+    float weight = 0.0f;
+    if (e < p.experts) {
+        if (tokens > 0)
+            weight = p.coef / static_cast<float>(p.sequences) * (static_cast<float>(p.experts) / (static_cast<float>(p.top) * n)) *
+                     (static_cast<float>(count) / n);
+        p.weights[static_cast<uint64_t>(s) * p.experts + e] = weight;
+        p.counts[static_cast<uint64_t>(s) * p.experts + e] = count;
+    }
+    float loss = weight * sum;
+#pragma unroll
+    for (uint32_t off = 16; off >= 1; off /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, off);
+    if (threadIdx.x == 0) p.losses[s * gridDim.x + blockIdx.x] = loss;
+}
+
+// Strips from the last to the first: what the first launch read last is what L2 still holds.
+template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
+__global__ void __launch_bounds__(kBalanceThreads) balance_grad_kernel(const BalanceParams p, uint32_t num_losses) {
+    using Row = detail::BalanceRow<T, kVec, kLanes, kIter>;
+    constexpr uint32_t kPerLane = Row::kPerLane;
+    ptx::grid_dependency_wait();
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (blockIdx.x == 0 && warp == 0) {
+        float loss = 0.0f;
+        for (uint32_t i = lane; i < num_losses; i += 32) loss += p.losses[i];
+#pragma unroll
+        for (uint32_t off = 16; off >= 1; off /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, off);
+        if (lane == 0) *p.loss = loss;
+    }
+    if (p.grad == nullptr) return;
+    const uint32_t strip = gridDim.x - 1 - blockIdx.x, first = strip * p.strip_tokens, last = min(first + p.strip_tokens, p.tokens);
+    const T* logits = static_cast<const T*>(p.logits);
+    T* grad = static_cast<T*>(p.grad);
+    float weights[kPerLane];
+    uint32_t at = first;  // tokens below have their gradient
+    for (uint32_t s = detail::first_sequence_behind(p, first); at < last; ++s) {
+        // the tokens up to the sequence belong to none: their gradient is zero
+        uint32_t begin = last, end = last;
+        if (s < p.sequences) detail::sequence_range(p, s, begin, end);
+        begin = min(max(begin, at), last), end = min(max(end, begin), last);
+        if (begin < end) {
+#pragma unroll
+            for (uint32_t c = 0; c < kPerLane; ++c) {
+                const uint32_t col = Row::column(lane, c);
+                weights[c] = col < p.experts ? p.weights[static_cast<uint64_t>(s) * p.experts + col] : 0.0f;
+            }
+        }
+        for (uint32_t base = at + warp * Row::kRowsPerWarp; base < end; base += kBalanceWarps * Row::kRowsPerWarp) {
+            const uint32_t token = base + lane / kLanes;
+            const bool counts = token >= begin && token < end && (p.mask == nullptr || p.mask[token] != 0);
+            float z[kPerLane];
+            Row::load(logits + static_cast<uint64_t>(token) * p.logits_ld, counts, p.experts, lane, z);
+            const float2 row = counts ? p.rows[token] : make_float2(0.0f, 0.0f);
+            Row::scores(p.sigmoid != 0, z, row.x);
+            float inner = 0.0f;
+#pragma unroll
+            for (uint32_t c = 0; c < kPerLane; ++c) inner = fmaf(z[c], weights[c], inner);
+            inner = Row::sum(inner) * row.y;
+#pragma unroll
+            for (uint32_t c = 0; c < kPerLane; ++c) {
+                const float slope = p.sigmoid != 0 ? z[c] * (1.0f - z[c]) : z[c];
+                z[c] = counts ? slope * row.y * (weights[c] - inner) : 0.0f;
+            }
+            if (token < end) Row::store(grad + static_cast<uint64_t>(token) * p.grad_ld, p.experts, lane, z);
+        }
+        at = end;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+struct BalanceWorkspace {
+    uint32_t strips, strip_tokens;
+    size_t sums, counts, tokens, weights, losses, rows, bytes;
+};
+
+inline BalanceWorkspace plan_balance_workspace(uint32_t tokens, uint32_t experts, uint32_t sequences, bool with_grad, uint32_t num_sms) {
+    BalanceWorkspace w;
+    // two CTAs per SM, at least four tokens per warp
+    w.strip_tokens = ceil_div(tokens, 2 * num_sms);
+    if (w.strip_tokens < 4 * kBalanceWarps) w.strip_tokens = 4 * kBalanceWarps;
+    w.strips = ceil_div(tokens, w.strip_tokens);
+    if (w.strips == 0) w.strips = 1;
+    const size_t slots = static_cast<size_t>(w.strips) + sequences;
+    size_t at = 0;
+    auto take = [&at](size_t bytes) {
+        const size_t here = at;
+        at = align_up(at + bytes, static_cast<size_t>(256));
+        return here;
+    };
+    w.sums = take(slots * experts * 4);
+    w.counts = take(slots * experts * 4);
+    w.tokens = take(slots * 4);
+    w.weights = take(static_cast<size_t>(sequences) * experts * 4);
+    w.losses = take(static_cast<size_t>(sequences) * ceil_div(experts, 32u) * 4);
+    w.rows = take(with_grad ? static_cast<size_t>(tokens) * 8 : 0);
+    w.bytes = at;
+    return w;
+}
+
+template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
+inline int launch_balance_as(const BalanceParams& p, cudaStream_t stream) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.strips);
+    cfg.blockDim = dim3(kBalanceThreads);
+    cfg.dynamicSmemBytes = kBalanceWarps * p.experts * sizeof(float);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, balance_sums_kernel<T, kVec, kLanes, kIter>, p);
+    cfg.dynamicSmemBytes = 0;
+    const uint32_t parts = ceil_div(p.experts, 32u);
+    cfg.gridDim = dim3(parts, p.sequences);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, balance_weights_kernel, p);
+    cfg.gridDim = dim3(p.grad != nullptr ? p.strips : 1u);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, balance_grad_kernel<T, kVec, kLanes, kIter>, p, parts * p.sequences);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return kLaunchFailed;
+    }
+    return kOk;
+}
+
+template <typename T>
+inline int launch_balance(const BalanceParams& p, cudaStream_t stream) {
+    constexpr uint32_t kVec = 16 / sizeof(T);
+    const bool vector = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && reinterpret_cast<uintptr_t>(p.grad) % 16 == 0 &&
+                        p.logits_ld % kVec == 0 && p.grad_ld % kVec == 0 && p.experts % kVec == 0;
+    if (vector) {
+        const uint32_t lanes = p.experts / kVec;
+        if (lanes <= 8) return launch_balance_as<T, kVec, 8, 1>(p, stream);
+        if (lanes <= 16) return launch_balance_as<T, kVec, 16, 1>(p, stream);
+        if (lanes <= 32) return launch_balance_as<T, kVec, 32, 1>(p, stream);
+        if (lanes <= 64) return launch_balance_as<T, kVec, 32, 2>(p, stream);
+        if (lanes <= 128) return launch_balance_as<T, kVec, 32, 4>(p, stream);
+        return launch_balance_as<T, kVec, 32, 1024 / kVec / 32>(p, stream);
+    }
+    if (p.experts <= 64) return launch_balance_as<T, 1, 32, 2>(p, stream);
+    if (p.experts <= 256) return launch_balance_as<T, 1, 32, 8>(p, stream);
+    return launch_balance_as<T, 1, 32, 32>(p, stream);
+}
+
+}  // namespace yan
