@@ -139,3 +139,16 @@ def test_python_operators_refuse(cuda_lib):
                      ((z(64, 1025, d=torch.float32), ids), {}), ((logits, ids), dict(workspace=z(8, d=torch.uint8)))]:
         with pytest.raises(AssertionError):
             yan_b200.moe_balance_loss(*args, **kw)
+
+
+def test_the_native_front_leaves_unusual_arguments_to_python():
+    from yan_b200 import _lib
+    f = _lib.fast()
+    t = torch.zeros(4, 8, dtype=torch.bfloat16)
+    assert f.wgrad(t, t, t, False, None, 148, None, None) == -1 and f.wgrad(t) == -1 and f.wgrad(1, 2, 3, 4, 5, 6, 7, 8) == -1
+    args = (0.1, None, None, 1e-3, 0.9, 0.99, 1e-8, 1)
+    assert f.adamw([t], [t], [t], [t], *args) == -1 and f.adamw([], [], [], [], *args) == -1 and f.adamw() == -1
+    assert f.adamw(t, t, t, t, *args) == -1 and f.adamw([t], [t, t], [t], [t], *args) == -1 and f.adamw([1], [None], ["x"], [t], *args) == -1
+    assert f.balance(t, t, None, None, 1.0, 0, 148) == -1 and f.balance() == -1 and f.balance("x", 1, 2, 3, 4, 5, 6) == -1
+    with pytest.raises(TypeError):
+        f.bind_train(1)

@@ -147,6 +147,10 @@ def fast():
         module.bind(*(ctypes.cast(getattr(handle, name), _P).value for name in
                       ("yan_b200_gemm_fp8_fp8_bf16_nt", "yan_b200_gemm_fp8_fp8_f32_nt", "yan_b200_fp8_linear_bf16",
                        "yan_b200_fp8_linear_workspace_bytes", "yan_b200_per_token_cast_to_fp8")))
+        module.bind_train(*(ctypes.cast(getattr(handle, name), _P).value for name in
+                            ("yan_b200_fp8_linear_wgrad_workspace_bytes", "yan_b200_fp8_linear_wgrad",
+                             "yan_b200_k_grouped_fp8_linear_wgrad", "yan_b200_adamw_step",
+                             "yan_b200_moe_balance_loss_workspace_bytes", "yan_b200_moe_balance_loss")))
         _fast = module
     return _fast
 

@@ -25,6 +25,7 @@ LIB_DIR = os.path.join(PKG_DIR, "lib")
 OBJ_DIR = os.path.join(PKG_DIR, "lib", "obj")
 LIB_PATH = os.path.join(LIB_DIR, "libyan_b200.so")
 FASTCALL_SRC = os.path.join(CSRC_DIR, "fastcall.cpp")
+FASTCALL_PARTS = (FASTCALL_SRC, os.path.join(CSRC_DIR, "fastcall_train.h"), os.path.join(os.path.dirname(PKG_DIR), "include", "yan_b200.h"))
 FASTCALL_PATH = os.path.join(LIB_DIR, "_fastcall.so")
 
 BLOCK_NS = (32, 64, 96, 128, 160, 192, 224, 256)
@@ -81,8 +82,11 @@ def build_fastcall(force: bool = False, verbose: bool = False) -> str:
     import torch
     from . import _lib
     torch_dir = os.path.dirname(torch.__file__)
-    with open(FASTCALL_SRC, "rb") as f:
-        key = f"{_lib.front_key()}{hashlib.sha256(f.read()).hexdigest()[:16]}|"
+    digest = hashlib.sha256()
+    for part in FASTCALL_PARTS:
+        with open(part, "rb") as f:
+            digest.update(f.read())
+    key = f"{_lib.front_key()}{digest.hexdigest()[:16]}|"
     if not force and _lib.front_built_for(key):
         return FASTCALL_PATH
     cxx = os.environ.get("CXX") or shutil.which("g++")

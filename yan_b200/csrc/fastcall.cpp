@@ -10,12 +10,16 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include "../../include/yan_b200.h"
 
 // What this file was compiled from and for, read out of the built file before it is loaded (front_key in _lib.py).
 extern "C" __attribute__((used)) const char yan_b200_front_key[] = YAN_FRONT_KEY;
@@ -216,11 +220,17 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Py_RETURN_NONE;
 }
 
+#include "fastcall_train.h"
+
 PyMethodDef g_methods[] = {
     {"gemm_bf16", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gemm<true>)), METH_FASTCALL, nullptr},
     {"gemm_f32", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gemm<false>)), METH_FASTCALL, nullptr},
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear)), METH_FASTCALL, nullptr},
     {"per_token_cast", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(per_token_cast)), METH_FASTCALL, nullptr},
+    {"wgrad", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(wgrad)), METH_FASTCALL, nullptr},
+    {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL, nullptr},
+    {"balance", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(balance)), METH_FASTCALL, nullptr},
+    {"bind_train", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_train)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

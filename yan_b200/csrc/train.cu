@@ -64,13 +64,14 @@ int adamw_some(const yan_b200_adamw_tensor* tensors, int first, int count, const
                bool grad_bf16, bool eight_bit, cudaStream_t stream, int* next) {
     yan::AdamwParams<kCapacity> p;
     p.s = scalars;
+    const uint32_t chunk = yan::adamw_chunk(eight_bit);
     uint32_t used = 0;
     uint64_t chunks = 0;
     int i = first;
     for (; i < count && used < kCapacity; ++i) {
         const yan_b200_adamw_tensor& t = tensors[i];
         if (t.numel == 0) continue;
-        const uint64_t more = (static_cast<uint64_t>(t.numel) + yan::kAdamwChunk - 1) / yan::kAdamwChunk;
+        const uint64_t more = (static_cast<uint64_t>(t.numel) + chunk - 1) / chunk;
         if (chunks + more > 0x7fffffffull) break;
         p.first_chunk[used] = static_cast<uint32_t>(chunks);
         yan::AdamwTensor& d = p.tensor[used];

@@ -36,6 +36,7 @@ static_assert(sizeof(AdamwTensor) == 72);
 struct AdamwScalars {
     const float* grad_scale;  // optional, on the device
     float b1, one_minus_b1, b2, one_minus_b2, step_size, inv_root_correction, eps;
+    float minus_zero = -0.0f;  // see rounded_product2
 };
 
 // The table of tensors travels with the launch (kernel parameters hold up to 32764 bytes), so that nothing about them has to be on the
@@ -50,8 +51,16 @@ struct AdamwParams {
 constexpr uint32_t kAdamwSmallCapacity = 48, kAdamwCapacity = 420;
 static_assert(sizeof(AdamwParams<kAdamwSmallCapacity>) <= 4096 && sizeof(AdamwParams<kAdamwCapacity>) <= 32764);
 
-constexpr uint32_t kAdamwThreads = 256, kAdamwBlocksPerWarp = 4;
-constexpr uint32_t kAdamwChunk = kAdamwThreads / 32 * kAdamwBlocksPerWarp * 128;  // elements of one CTA
+// A CTA is 256 threads whose warps take kBlocksPerWarp blocks of 128 elements each, all loads in flight together.  8-bit states bring
+// fewer bytes per element and need more of them in flight: us for (200 M elements in 64 tensors, 12 M in 300) with one block 633, 39;
+// two 591, 37; four at 64 registers per thread 532, 39 and at 80 648, 46; eight 526, 57.  32-bit states: (120 M elements in 12 tensors,
+// 120 thousand in 48) with one block 523, 2.9; two 525, 3.4; four 523, 4.9.
+template <bool k8Bit>
+struct AdamwShape {
+    static constexpr uint32_t kThreads = 256, kBlocksPerWarp = k8Bit ? 4 : 1, kMinCtas = k8Bit ? 4 : 1;
+    static constexpr uint32_t kChunk = kThreads / 32 * kBlocksPerWarp * 128;  // elements of one CTA
+};
+constexpr uint32_t adamw_chunk(bool eight_bit) { return eight_bit ? AdamwShape<true>::kChunk : AdamwShape<false>::kChunk; }
 
 namespace detail {
 
@@ -96,6 +105,15 @@ __device__ __forceinline__ void decode4(uint32_t codes, float scale, float (&f)[
     f[0] = a.x * scale, f[1] = a.y * scale, f[2] = b.x * scale, f[3] = b.y * scale;
 }
 
+// The power of two of a block and its reciprocal from the bits of its largest magnitude (finite): adding 0x1FFFFF carries into the exponent
+// exactly where the significand is above 1.75.
+__device__ __forceinline__ void block_scale(uint32_t amax, float& scale, float& inverse) {
+    const uint32_t bits = ((amax + 0x1FFFFFu) & 0x7F800000u) - (8u << 23);
+    const bool known = amax >= (16u << 23);
+    scale = known ? __uint_as_float(bits) : 0.0f;
+    inverse = known ? __uint_as_float((254u << 23) - bits) : 0.0f;
+}
+
 // Codes of a warp's block of 128, four elements per lane, and its power of two.  Called by whole warps.
 template <bool kRoot>
 __device__ __forceinline__ uint32_t encode4(const float (&f)[4], float& scale) {
@@ -108,11 +126,9 @@ __device__ __forceinline__ uint32_t encode4(const float (&f)[4], float& scale) {
         amax = max(amax, finite[j] ? magnitude : 0u);
     }
     amax = __reduce_max_sync(0xffffffffu, amax);
-    const bool known = amax >= (16u << 23);
-    const uint32_t e = (amax >> 23) - 8u + ((amax & 0x7FFFFFu) > 0x600000u ? 1u : 0u);
-    scale = known ? __uint_as_float(e << 23) : 0.0f;
-    const float inverse = known ? __uint_as_float((254u - e) << 23) : 0.0f;
-    const float smallest = known ? 0.001953125f : 0.0f;  // code 1
+    float inverse;
+    block_scale(amax, scale, inverse);
+    const float smallest = scale != 0.0f ? 0.001953125f : 0.0f;  // code 1
     float t[4];
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
@@ -142,12 +158,112 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint64_t i, uint32_t cou
         if (j < count) p[i + j] = static_cast<uint8_t>(codes >> (8 * j));
 }
 
+// Two fp32 operations with one instruction, each rounded like the single one.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// A product that is rounded by itself: a product of two feeds an addition of two as one fused operation, whatever rounding the
+// instructions name (1.6 of 16.8 million sums came out differently); an fma onto a -0 that the compiler does not know is not fused again.
+__device__ __forceinline__ uint64_t rounded_product2(uint64_t a, uint64_t b, float minus_zero) {
+    return fma2(a, b, pack2(minus_zero, minus_zero));
+}
+__device__ __forceinline__ float approximate_rsqrt(float x) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float approximate_reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// One block of 128 elements, four per lane, 8-bit states: updates param, codes and scales in registers.  The same operations as the general
+// form below, two at a time; the root by one Newton step from the hardware's reciprocal root in the form of Markstein (s = v y,
+// s + (v - s^2) y / 2), which rounds like sqrt for what is finite.  Returns false, with nothing changed, if an m or v is not finite.
+__device__ __forceinline__ bool update_block_8bit(const AdamwScalars& c, float grad_scale, float decay, float (&param)[4], const float (&grad)[4],
+                                                  uint32_t& m_codes, uint32_t& v_codes, float& m_scale, float& v_scale) {
+    float md[4], rd[4];
+    decode4(m_codes, m_scale, md);
+    decode4(v_codes, v_scale, rd);
+    uint64_t m[2], v[2], root[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint64_t g = mul2(pack2(grad[2 * h], grad[2 * h + 1]), pack2(grad_scale, grad_scale));
+        const uint64_t old_root = pack2(rd[2 * h], rd[2 * h + 1]);
+        m[h] = add2(rounded_product2(pack2(md[2 * h], md[2 * h + 1]), pack2(c.b1, c.b1), c.minus_zero),
+                    rounded_product2(g, pack2(c.one_minus_b1, c.one_minus_b1), c.minus_zero));
+        v[h] = add2(rounded_product2(mul2(old_root, old_root), pack2(c.b2, c.b2), c.minus_zero),
+                    rounded_product2(mul2(g, g), pack2(c.one_minus_b2, c.one_minus_b2), c.minus_zero));
+        float a, b;
+        unpack2(v[h], a, b);
+        // zero: s = 0 * y and its correction are zero, whatever the y
+        const uint64_t y = pack2(approximate_rsqrt(fmaxf(a, 1.2e-38f)), approximate_rsqrt(fmaxf(b, 1.2e-38f)));
+        const uint64_t s = mul2(v[h], y), minus_s = mul2(s, pack2(-1.0f, -1.0f));
+        root[h] = fma2(fma2(minus_s, s, v[h]), mul2(y, pack2(0.5f, 0.5f)), s);
+    }
+    float ma[4], ra[4], va[4];
+    unpack2(m[0], ma[0], ma[1]), unpack2(m[1], ma[2], ma[3]);
+    unpack2(root[0], ra[0], ra[1]), unpack2(root[1], ra[2], ra[3]);
+    unpack2(v[0], va[0], va[1]), unpack2(v[1], va[2], va[3]);
+    const float m_top = max_or_nan(max_or_nan(fabsf(ma[0]), fabsf(ma[1])), max_or_nan(fabsf(ma[2]), fabsf(ma[3])));
+    const float r_top = max_or_nan(max_or_nan(ra[0], ra[1]), max_or_nan(ra[2], ra[3]));  // NaN where v is not finite
+    const uint32_t m_amax = __reduce_max_sync(0xffffffffu, __float_as_uint(m_top) & 0x7FFFFFFFu);
+    const uint32_t r_amax = __reduce_max_sync(0xffffffffu, __float_as_uint(r_top) & 0x7FFFFFFFu);
+    if (max(m_amax, r_amax) >= 0x7F800000u) return false;
+    float m_inverse, r_inverse;
+    block_scale(m_amax, m_scale, m_inverse);
+    block_scale(r_amax, v_scale, r_inverse);
+    const float smallest = v_scale != 0.0f ? 0.001953125f : 0.0f;  // code 1
+    uint32_t mw[2], rw[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        float a, b;
+        unpack2(mul2(m[h], pack2(m_inverse, m_inverse)), a, b);
+        mw[h] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        unpack2(mul2(root[h], pack2(r_inverse, r_inverse)), a, b);
+        a = fmaxf(a, ra[2 * h] > 0.0f ? smallest : 0.0f), b = fmaxf(b, ra[2 * h + 1] > 0.0f ? smallest : 0.0f);
+        rw[h] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        const uint64_t denominator = fma2(root[h], pack2(c.inv_root_correction, c.inv_root_correction), pack2(c.eps, c.eps));
+        unpack2(denominator, a, b);
+        const uint64_t step = mul2(m[h], pack2(-c.step_size, -c.step_size));
+        const uint64_t kept = mul2(pack2(param[2 * h], param[2 * h + 1]), pack2(decay, decay));
+        unpack2(fma2(step, pack2(approximate_reciprocal(a), approximate_reciprocal(b)), kept), param[2 * h], param[2 * h + 1]);
+    }
+    m_codes = mw[0] | (mw[1] << 16);
+    v_codes = rw[0] | (rw[1] << 16);
+    return true;
+}
+
 }  // namespace detail
 
-// One CTA per chunk; a warp takes kAdamwBlocksPerWarp blocks of 128 elements, four elements per lane each, and has their loads in
-// flight together.
+// One CTA per chunk of a tensor, four elements of a block per lane.
 template <typename param_t, typename grad_t, bool k8Bit, uint32_t kCapacity>
-__global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const __grid_constant__ AdamwParams<kCapacity> p) {
+__global__ void __launch_bounds__(AdamwShape<k8Bit>::kThreads, AdamwShape<k8Bit>::kMinCtas) adamw_kernel(const __grid_constant__ AdamwParams<kCapacity> p) {
+    constexpr uint32_t kBlocks = AdamwShape<k8Bit>::kBlocksPerWarp;
     ptx::grid_dependency_wait();
     uint32_t low = 0, high = p.num_tensors;  // first_chunk[low] <= blockIdx.x < first_chunk[high]
     while (high - low > 1) {
@@ -159,17 +275,55 @@ __global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const __grid_const
     const uint64_t numel = t.numel_lo | (static_cast<uint64_t>(t.numel_hi) << 32);
     const bool vector = t.vector != 0;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint64_t start = static_cast<uint64_t>(blockIdx.x - p.first_chunk[low]) * kAdamwChunk + warp * (kAdamwBlocksPerWarp * 128u) + lane * 4u;
+    const uint64_t start = static_cast<uint64_t>(blockIdx.x - p.first_chunk[low]) * AdamwShape<k8Bit>::kChunk + warp * (kBlocks * 128u) + lane * 4u;
     param_t* param = static_cast<param_t*>(t.param);
     const grad_t* grad = static_cast<const grad_t*>(t.grad);
     const float grad_scale = p.s.grad_scale != nullptr ? *p.s.grad_scale : 1.0f;
 
-    float pv[kAdamwBlocksPerWarp][4], g[kAdamwBlocksPerWarp][4], m[kAdamwBlocksPerWarp][4], v[kAdamwBlocksPerWarp][4];
-    uint32_t count[kAdamwBlocksPerWarp];
-    [[maybe_unused]] uint32_t mc[kAdamwBlocksPerWarp], vc[kAdamwBlocksPerWarp];
-    [[maybe_unused]] float ms[kAdamwBlocksPerWarp], vs[kAdamwBlocksPerWarp];
+    [[maybe_unused]] uint32_t todo = (1u << kBlocks) - 1;  // blocks for the general form
+    if constexpr (k8Bit) {
+        // Whole blocks of a tensor whose pointers allow four elements at a time.  What bounds it is the number of instructions: written
+        // like the general form below, 371 per 128 elements, 200 M elements took 957 us.
+        if (vector && start - lane * 4u + kBlocks * 128u <= numel) {
+            param_t* pp = param + start;
+            const grad_t* gp = grad + start;
+            uint8_t *mp = static_cast<uint8_t*>(t.m) + start, *vp = static_cast<uint8_t*>(t.v) + start;
+            float *msp = t.m_scale + start / 128u, *vsp = t.v_scale + start / 128u;
+            __nv_bfloat16* cp = t.copy;
+            float pv[kBlocks][4], g[kBlocks][4], ms[kBlocks], vs[kBlocks];
+            uint32_t mc[kBlocks], vc[kBlocks];
 #pragma unroll
-    for (uint32_t b = 0; b < kAdamwBlocksPerWarp; ++b) {
+            for (uint32_t b = 0; b < kBlocks; ++b) {
+                detail::load4(pp, b * 128u, 4, true, pv[b]);
+                detail::load4(gp, b * 128u, 4, true, g[b]);
+                mc[b] = detail::load_codes(mp, b * 128u, 4, true);
+                vc[b] = detail::load_codes(vp, b * 128u, 4, true);
+                ms[b] = msp[b];
+                vs[b] = vsp[b];
+            }
+#pragma unroll
+            for (uint32_t b = 0; b < kBlocks; ++b) {
+                if (!detail::update_block_8bit(p.s, grad_scale, t.decay, pv[b], g[b], mc[b], vc[b], ms[b], vs[b])) continue;
+                todo &= ~(1u << b);
+                detail::store4(pp, b * 128u, 4, true, pv[b]);
+                if (cp != nullptr) detail::store4(cp, start + b * 128u, 4, true, pv[b]);
+                detail::store_codes(mp, b * 128u, 4, true, mc[b]);
+                detail::store_codes(vp, b * 128u, 4, true, vc[b]);
+                if (lane == 0) {
+                    msp[b] = ms[b];
+                    vsp[b] = vs[b];
+                }
+            }
+            if (todo == 0) return;  // otherwise something is not finite there
+        }
+    }
+    float pv[kBlocks][4], g[kBlocks][4], m[kBlocks][4], v[kBlocks][4];
+    uint32_t count[kBlocks];
+    [[maybe_unused]] uint32_t mc[kBlocks], vc[kBlocks];
+    [[maybe_unused]] float ms[kBlocks], vs[kBlocks];
+#pragma unroll
+    for (uint32_t b = 0; b < kBlocks; ++b) {
+        if (k8Bit && (todo >> b & 1u) == 0) continue;
         const uint64_t i = start + b * 128u;
         count[b] = i < numel ? static_cast<uint32_t>(min(numel - i, static_cast<uint64_t>(4))) : 0u;
         detail::load4(param, i, count[b], vector, pv[b]);
@@ -186,7 +340,8 @@ __global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const __grid_const
         }
     }
 #pragma unroll
-    for (uint32_t b = 0; b < kAdamwBlocksPerWarp; ++b) {
+    for (uint32_t b = 0; b < kBlocks; ++b) {
+        if (k8Bit && (todo >> b & 1u) == 0) continue;
         const uint64_t i = start + b * 128u;
         if constexpr (k8Bit) {
             detail::decode4(mc[b], ms[b], m[b]);
@@ -200,8 +355,8 @@ __global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const __grid_const
             m[b][j] = __fadd_rn(__fmul_rn(m[b][j], p.s.b1), __fmul_rn(gj, p.s.one_minus_b1));
             v[b][j] = __fadd_rn(__fmul_rn(v[b][j], p.s.b2), __fmul_rn(__fmul_rn(gj, gj), p.s.one_minus_b2));
             root[j] = __fsqrt_rn(v[b][j]);
-            const float update = __fdividef(m[b][j] * p.s.step_size, fmaf(root[j], p.s.inv_root_correction, p.s.eps));
-            pv[b][j] = fmaf(pv[b][j], t.decay, -update);
+            const float reciprocal = detail::approximate_reciprocal(fmaf(root[j], p.s.inv_root_correction, p.s.eps));
+            pv[b][j] = fmaf(__fmul_rn(m[b][j], -p.s.step_size), reciprocal, __fmul_rn(pv[b][j], t.decay));
         }
         detail::store4(param, i, count[b], vector, pv[b]);
         if (t.copy != nullptr) detail::store4(t.copy, i, count[b], vector, pv[b]);
@@ -231,7 +386,7 @@ inline int launch_adamw_as(const AdamwParams<kCapacity>& p, cudaStream_t stream)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.first_chunk[p.num_tensors]);
-    cfg.blockDim = dim3(kAdamwThreads);
+    cfg.blockDim = dim3(AdamwShape<k8Bit>::kThreads);
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;

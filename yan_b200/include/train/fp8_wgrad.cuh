@@ -160,26 +160,45 @@ struct WgradParams {
     void* out = nullptr;                  // [groups][n][out_ld]
     uint64_t out_ld = 0, out_group = 0;   // elements
     uint32_t accumulate = 0;
-    uint32_t vector_store = 0;            // rows of dW start on 16-byte boundaries and have whole vectors
-    // The tokens of every tile shared by `slices` CTAs: each writes its partial tile, the last one adds them in order.
-    uint32_t slices = 1;
-    float4* partials = nullptr;           // [tile][slice][8 warps][32][32 lanes] float4
-    uint32_t* counters = nullptr;         // [tile][8 warps]
+    uint32_t vector_store = 0;            // rows of dW allow four elements at a time
+    uint32_t tiles = 0, whole_tiles = 0;  // all of them; those that are dealt out one by one (see WgradSchedule)
+    uint32_t store_cost = 0;              // k-blocks that take as long as storing a tile
+    float4* partials = nullptr;           // [2 * CTAs][8 warps][32][32 lanes]
+    uint32_t* counters = nullptr;         // [CTAs][8 warps], zero
     int* status = nullptr;
     unsigned long long timeout_ns = 0;
+};
+
+// Who computes what.  Tiles are numbered group by group, within a group in bands of 16 tile rows, so that CTAs at work at the same time
+// share what they read.  The first whole_tiles of them, a multiple of the CTAs, are dealt out in turn.  The rest, less than two waves,
+// is shared evenly: laid end to end, a tile as long as its k-blocks or as its store takes, whichever is more, and cut into one
+// stretch per CTA.  A cut through the k-blocks of a tile goes to a multiple of four of them; tiles of fewer than kMinCut go whole to
+// the CTA in whose stretch they begin.
+struct WgradSchedule {
+    TokenBlockTable blocks;
+    uint64_t length[kMaxTokenGroups + 1];  // of all tiles in front of a group
+    uint64_t origin, rest;                 // where the shared tiles begin, and their length
+    uint32_t stretches;
 };
 
 struct WgradTile {
     static constexpr uint32_t kBlockFeatures = 256;  // columns of a tile (features of x); its rows are 128 features of dy
     static constexpr uint32_t kStages = 4;
+    // k-blocks that are summed in tensor memory before the sums move to registers.  An addition there rounds towards zero (8192 tokens of
+    // uneven size, relative error: 1.3e-6 in one chain).
+#ifndef YAN_WGRAD_CHAIN
+#define YAN_WGRAD_CHAIN 32
+#endif
+    static constexpr uint32_t kChain = YAN_WGRAD_CHAIN;
+    static constexpr uint32_t kMinCut = 8, kMinStretch = 8;
     static constexpr uint32_t kStageA = kMnBoxBytes, kStageB = 2 * kMnBoxBytes;
     static constexpr uint32_t kScaleTiles = 1 + kBlockFeatures / 128;
     static constexpr uint32_t kStageScales = kScaleTiles * kScaleTileBytes;
     static constexpr uint32_t kOffA = 0, kOffB = kOffA + kStages * kStageA, kOffScales = kOffB + kStages * kStageB;
     static constexpr uint32_t kBoxRowBytes = 64, kBoxBytes = 32 * kBoxRowBytes;  // output staging, one box per warp
     static constexpr uint32_t kOffStore = kOffScales + kStages * kStageScales;
-    static constexpr uint32_t kOffTable = kOffStore + 8 * kBoxBytes;
-    static constexpr uint32_t kOffBarriers = align_up(kOffTable + static_cast<uint32_t>(sizeof(TokenBlockTable)), 8u);
+    static constexpr uint32_t kOffSchedule = kOffStore + 8 * kBoxBytes;
+    static constexpr uint32_t kOffBarriers = align_up(kOffSchedule + static_cast<uint32_t>(sizeof(WgradSchedule)), 8u);
     static constexpr uint32_t kNumBarriers = 2 * kStages + 2;
     static constexpr uint32_t kOffTmemSlot = kOffBarriers + kNumBarriers * 8, kOffAbort = kOffTmemSlot + 4;
     static constexpr uint32_t kSmemSize = kOffAbort + 4 + 1024;
@@ -187,63 +206,158 @@ struct WgradTile {
     static constexpr uint32_t kTmemScales = kBlockFeatures, kTmemScaleSet = kScaleTiles * 4, kTmemCols = 512;
     static_assert(kTmemScales + 2 * kTmemScaleSet <= kTmemCols);
     static_assert(kSmemSize <= 232448);
+    static_assert(kChain % 4 == 0 && kMinCut % 4 == 0 && kMinStretch >= 8);
 };
 
 namespace detail {
 
-// What one CTA computes at a time: k-blocks (128 tokens) [begin, begin + count) of a group for one tile of its dW.
+__device__ __forceinline__ uint32_t wgrad_tiles_per_group(const WgradParams& p) {
+    return ceil_div(p.n, 128u) * ceil_div(p.k, WgradTile::kBlockFeatures);
+}
+// Length of a tile with so many k-blocks.  Nothing is left to do for an empty group that is added.
+__device__ __forceinline__ uint32_t wgrad_length(const WgradParams& p, uint32_t blocks) {
+    return blocks == 0 && p.accumulate != 0 ? 0u : max(blocks, p.store_cost);
+}
+
+// Called by one whole warp.
+__device__ __forceinline__ void build_wgrad_schedule(const WgradParams& p, WgradSchedule& s) {
+    build_token_blocks(p.groups, p.max_blocks, s.blocks);
+    const uint32_t lane = ptx::lane_id(), per_group = wgrad_tiles_per_group(p);
+    uint64_t at = 0;
+    for (uint32_t first = 0; first < p.groups.num_groups; first += 32) {
+        const uint32_t g = first + lane;
+        const uint64_t own = g < p.groups.num_groups
+                                 ? static_cast<uint64_t>(per_group) * wgrad_length(p, s.blocks.block[g + 1] - s.blocks.block[g]) : 0u;
+        uint64_t until = own;
+#pragma unroll
+        for (uint32_t off = 1; off < 32; off *= 2) {
+            const uint64_t v = __shfl_up_sync(0xffffffffu, until, off);
+            if (lane >= off) until += v;
+        }
+        if (g < p.groups.num_groups) s.length[g] = at + until - own;
+        at += __shfl_sync(0xffffffffu, until, 31);
+    }
+    __syncwarp();
+    if (lane == 0) {
+        s.length[p.groups.num_groups] = at;
+        const uint32_t g = p.whole_tiles / per_group;
+        s.origin = at;
+        if (g < p.groups.num_groups)
+            s.origin = s.length[g] + static_cast<uint64_t>(p.whole_tiles % per_group) * wgrad_length(p, s.blocks.block[g + 1] - s.blocks.block[g]);
+        s.rest = at - s.origin;
+        s.stretches = static_cast<uint32_t>(max(min(static_cast<uint64_t>(gridDim.x), s.rest / WgradTile::kMinStretch), static_cast<uint64_t>(1)));
+    }
+}
+
+// What one CTA computes at a time: k-blocks [begin, begin + count) of a group, of `blocks`, for one tile of its dW.
 struct WgradUnit {
-    uint32_t group, row0, col0, tile, slice;  // row0, col0: features of the tile's corner
-    uint32_t block0;                          // first k-block among those of all groups (128 rows of codes each)
-    uint32_t quad0;                           // the group's first quad of scales
-    uint32_t begin, count;                    // within the group
+    uint32_t group, row0, col0;        // row0, col0: features of the tile's corner
+    uint32_t block0, quad0;            // the group's first k-block and quad of scales
+    uint32_t begin, count, blocks;
+    uint32_t first_cta, last_cta;      // who shares the tile
 };
 
-// Units are numbered slice by slice, tile by tile, group by group; tiles in bands of 16 tile rows, so that CTAs at work at the same
-// time share what they read.
-__device__ __forceinline__ bool get_wgrad_unit(const WgradParams& p, const TokenBlockTable& table, uint32_t index, WgradUnit& u) {
-    const uint32_t tiles_n = ceil_div(p.n, 128u), tiles_k = ceil_div(p.k, WgradTile::kBlockFeatures), per_group = tiles_n * tiles_k;
-    u.tile = index / p.slices;
-    u.slice = index % p.slices;
-    u.group = u.tile / per_group;
-    if (u.group >= p.groups.num_groups) return false;
-    const uint32_t t = u.tile % per_group, band = t / (16 * tiles_k), in_band = t % (16 * tiles_k), rows = min(16u, tiles_n - band * 16);
-    u.row0 = (band * 16 + in_band % rows) * 128;
-    u.col0 = in_band / rows * WgradTile::kBlockFeatures;
-    const uint32_t blocks = table.block[u.group + 1] - table.block[u.group];
-    u.block0 = table.block[u.group];
-    u.quad0 = table.quad[u.group];
-    u.begin = static_cast<uint64_t>(u.slice) * blocks / p.slices;
-    u.count = static_cast<uint64_t>(u.slice + 1) * blocks / p.slices - u.begin;
-    return true;
-}
+// The CTA's units one after the other; every role of the CTA walks them.
+struct WgradWalk {
+    uint32_t tile;        // next of the dealt tiles
+    uint64_t at, end;     // what is left of the CTA's stretch
 
-template <typename out_t>
-__device__ __forceinline__ uint4 add_to(uint4 v, uint4 old) {
-    if constexpr (sizeof(out_t) == 4) {
-        v.x = __float_as_uint(__uint_as_float(v.x) + __uint_as_float(old.x));
-        v.y = __float_as_uint(__uint_as_float(v.y) + __uint_as_float(old.y));
-        v.z = __float_as_uint(__uint_as_float(v.z) + __uint_as_float(old.z));
-        v.w = __float_as_uint(__uint_as_float(v.w) + __uint_as_float(old.w));
+    __device__ __forceinline__ explicit WgradWalk(const WgradSchedule& s)
+        : tile(blockIdx.x),
+          at(blockIdx.x < s.stretches ? s.origin + blockIdx.x * s.rest / s.stretches : 0u),
+          end(blockIdx.x < s.stretches ? s.origin + (blockIdx.x + 1u) * s.rest / s.stretches : 0u) {}
+
+    __device__ __forceinline__ static void place(const WgradParams& p, const WgradSchedule& s, uint32_t group, uint32_t in_group, WgradUnit& u) {
+        const uint32_t tiles_n = ceil_div(p.n, 128u), tiles_k = ceil_div(p.k, WgradTile::kBlockFeatures);
+        const uint32_t band = in_group / (16 * tiles_k), in_band = in_group % (16 * tiles_k), rows = min(16u, tiles_n - band * 16);
+        u.group = group;
+        u.row0 = (band * 16 + in_band % rows) * 128;
+        u.col0 = in_band / rows * WgradTile::kBlockFeatures;
+        u.block0 = s.blocks.block[group];
+        u.quad0 = s.blocks.quad[group];
+        u.blocks = s.blocks.block[group + 1] - u.block0;
     }
-    return v;
-}
+    // The CTA in whose stretch a position lies.
+    __device__ __forceinline__ static uint32_t owner(const WgradSchedule& s, uint64_t position) {
+        return static_cast<uint32_t>(((position - s.origin + 1) * s.stretches - 1) / s.rest);
+    }
+
+    __device__ __forceinline__ bool next(const WgradParams& p, const WgradSchedule& s, WgradUnit& u) {
+        const uint32_t per_group = wgrad_tiles_per_group(p);
+        if (tile < p.whole_tiles) {
+            place(p, s, tile / per_group, tile % per_group, u);
+            u.begin = 0, u.count = u.blocks;
+            u.first_cta = u.last_cta = blockIdx.x;
+            tile += gridDim.x;
+            return true;
+        }
+        while (at < end) {
+            uint32_t low = 0, high = p.groups.num_groups;  // length[low] <= at < length[high]
+            while (high - low > 1) {
+                const uint32_t mid = (low + high) / 2;
+                if (s.length[mid] <= at) low = mid;
+                else high = mid;
+            }
+            const uint32_t blocks = s.blocks.block[low + 1] - s.blocks.block[low], length = wgrad_length(p, blocks);
+            const uint32_t in_group = static_cast<uint32_t>((at - s.length[low]) / length);
+            const uint64_t start = s.length[low] + static_cast<uint64_t>(in_group) * length;
+            const uint32_t from = static_cast<uint32_t>(at - start);  // above zero only in the tile that the stretch begins in
+            const uint64_t until = end - start;
+            at = start + length;
+            place(p, s, low, in_group, u);
+            if (blocks < WgradTile::kMinCut) {
+                if (from != 0) continue;
+                u.begin = 0, u.count = blocks;
+                u.first_cta = u.last_cta = blockIdx.x;
+                return true;
+            }
+            u.begin = from >= blocks ? blocks : from & ~3u;
+            u.count = (until >= blocks ? blocks : static_cast<uint32_t>(until) & ~3u) - u.begin;
+            if (u.count == 0) continue;
+            u.first_cta = owner(s, start + 3);  // a stretch that ends in the first three k-blocks has none of them
+            u.last_cta = owner(s, start + blocks - 1);
+            return true;
+        }
+        return false;
+    }
+};
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 
-// Stores a warp's 32 rows x 128 columns; lane r holds row r.  The rows go through the warp's box in shared memory, 64 bytes of each at
-// a time in fp32, so that a store instruction covers eight pieces of 64 contiguous bytes.  Old values of a bf16 output are added in
-// 32 bits as well: the box holds fp32 in either case and the sum is rounded once.
+__device__ __forceinline__ void red_add(float* p, float v) { asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory"); }
+__device__ __forceinline__ void red_add4(float* p, const uint4& v) {
+    asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(__uint_as_float(v.x)), "f"(__uint_as_float(v.y)),
+                 "f"(__uint_as_float(v.z)), "f"(__uint_as_float(v.w))
+                 : "memory");
+}
+
+// Stores a warp's 32 rows x 128 columns; lane r holds row r.  The rows go through the warp's box in shared memory, 16 columns at a time in
+// fp32, so that a store instruction covers eight pieces of 64 contiguous bytes.  fp32 is added to what dW holds where dW lies, in L2:
+// every element once, so that the order does not matter, and nothing waits for the old value (16 experts N=4096 K=2048, 16384 tokens:
+// 535 us with loads and stores).  bf16 is loaded, added in 32 bits and rounded once.
 template <typename out_t>
 __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const WgradUnit& u, uint32_t box, uint32_t row_in_tile, uint32_t col0,
                                                  uint32_t lane, const float (&acc)[128]) {
     out_t* out = reinterpret_cast<out_t*>(p.out) + u.group * p.out_group;
     const uint32_t row0 = u.row0 + row_in_tile;
+    if (u.col0 + col0 >= p.k || row0 >= p.n) return;
 #pragma unroll
     for (uint32_t pass = 0; pass < 8; ++pass) {
+        const uint32_t chunk = lane % 4, col = u.col0 + col0 + pass * 16 + chunk * 4;
+        [[maybe_unused]] uint2 old[4];
+        if constexpr (sizeof(out_t) == 2) {
+            if (p.vector_store != 0 && p.accumulate != 0) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t r = row0 + i * 8 + lane / 4;
+                    old[i] = make_uint2(0, 0);
+                    if (r < p.n && col < p.k) old[i] = *reinterpret_cast<const uint2*>(out + static_cast<uint64_t>(r) * p.out_ld + col);
+                }
+            }
+        }
         __syncwarp();  // the read-back of the previous pass is over
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
@@ -252,39 +366,40 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
                               make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3])));
         }
         __syncwarp();
-        const uint32_t chunk = lane % 4, col = u.col0 + col0 + pass * 16 + chunk * 4;
+        if (p.vector_store != 0) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t r = i * 8 + lane / 4;
-            uint4 v = ptx::ld_shared_v4(box + r * 64 + ((chunk ^ ((r >> 1) & 3u)) << 4));
-            if (row0 + r >= p.n || col >= p.k) continue;
-            out_t* dst = out + static_cast<uint64_t>(row0 + r) * p.out_ld + col;
-            if (p.vector_store != 0) {
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t r = i * 8 + lane / 4;
+                uint4 v = ptx::ld_shared_v4(box + r * 64 + ((chunk ^ ((r >> 1) & 3u)) << 4));
+                if (row0 + r >= p.n || col >= p.k) continue;
+                out_t* dst = out + static_cast<uint64_t>(row0 + r) * p.out_ld + col;
                 if constexpr (sizeof(out_t) == 4) {
-                    if (p.accumulate != 0) v = add_to<out_t>(v, *reinterpret_cast<const uint4*>(dst));
-                    *reinterpret_cast<uint4*>(dst) = v;
+                    if (p.accumulate != 0) red_add4(dst, v);
+                    else *reinterpret_cast<uint4*>(dst) = v;
                 } else {
                     if (p.accumulate != 0) {
-                        const uint2 old = *reinterpret_cast<const uint2*>(dst);
-                        v.x = __float_as_uint(__uint_as_float(v.x) + __uint_as_float(old.x << 16));
-                        v.y = __float_as_uint(__uint_as_float(v.y) + __uint_as_float(old.x & 0xFFFF0000u));
-                        v.z = __float_as_uint(__uint_as_float(v.z) + __uint_as_float(old.y << 16));
-                        v.w = __float_as_uint(__uint_as_float(v.w) + __uint_as_float(old.y & 0xFFFF0000u));
+                        v.x = __float_as_uint(__uint_as_float(v.x) + __uint_as_float(old[i].x << 16));
+                        v.y = __float_as_uint(__uint_as_float(v.y) + __uint_as_float(old[i].x & 0xFFFF0000u));
+                        v.z = __float_as_uint(__uint_as_float(v.z) + __uint_as_float(old[i].y << 16));
+                        v.w = __float_as_uint(__uint_as_float(v.w) + __uint_as_float(old[i].y & 0xFFFF0000u));
                     }
                     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(__uint_as_float(v.x), __uint_as_float(v.y)),
                                                                 pack_bf16(__uint_as_float(v.z), __uint_as_float(v.w)));
                 }
-            } else {
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (uint32_t c = 0; c < 4; ++c) {
-                    if (col + c >= p.k) continue;
-                    float f = __uint_as_float(w[c]);
-                    if constexpr (sizeof(out_t) == 4) {
-                        dst[c] = p.accumulate != 0 ? f + dst[c] : f;
-                    } else {
-                        dst[c] = __float2bfloat16_rn(p.accumulate != 0 ? f + __bfloat162float(dst[c]) : f);
-                    }
+            }
+        } else {
+            // one element per lane, two rows at a time
+            const uint32_t c = lane % 16, column = u.col0 + col0 + pass * 16 + c;
+#pragma unroll 4
+            for (uint32_t r = lane / 16; r < 32; r += 2) {
+                const float v = ptx::ld_shared_f32(box + r * 64 + (((c / 4) ^ ((r >> 1) & 3u)) << 4) + c % 4 * 4);
+                if (row0 + r >= p.n || column >= p.k) continue;
+                out_t* dst = out + static_cast<uint64_t>(row0 + r) * p.out_ld + column;
+                if constexpr (sizeof(out_t) == 4) {
+                    if (p.accumulate != 0) red_add(dst, v);
+                    else *dst = v;
+                } else {
+                    *dst = __float2bfloat16_rn(p.accumulate != 0 ? v + __bfloat162float(*dst) : v);
                 }
             }
         }
@@ -300,7 +415,7 @@ __global__ void __launch_bounds__(384, 1)
     using T = WgradTile;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
-    TokenBlockTable& table = *reinterpret_cast<TokenBlockTable*>(smem + T::kOffTable);
+    WgradSchedule& schedule = *reinterpret_cast<WgradSchedule*>(smem + T::kOffSchedule);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + T::kOffBarriers);
     uint64_t* empty = full + T::kStages;
     uint64_t* sums_full = empty + T::kStages;
@@ -326,7 +441,7 @@ __global__ void __launch_bounds__(384, 1)
         ptx::fence_proxy_async_smem();
     }
     ptx::grid_dependency_wait();
-    if (warp == 3) build_token_blocks(p.groups, p.max_blocks, table);
+    if (warp == 3) detail::build_wgrad_schedule(p, schedule);
     if (warp == 2) {
         ptx::tmem_alloc(tmem_slot, T::kTmemCols);
         ptx::tmem_relinquish_alloc_permit();
@@ -336,16 +451,18 @@ __global__ void __launch_bounds__(384, 1)
     ptx::tcgen05_fence_after_thread_sync();
     const uint32_t tmem = *tmem_slot;
     const uint32_t tiles_n = ceil_div(p.n, 128u), tiles_k128 = ceil_div(p.k, 128u);
+    detail::WgradWalk walk(schedule);
+    detail::WgradUnit u;
 
     if (warp < 4) {
-        ptx::reg_dealloc<40>();
+        ptx::reg_dealloc<56>();
         if (warp == 0 && lane == 0) {
             // ---- loads: a k-block of both operands per stage, and the scales of four k-blocks with the first of them ----
             uint32_t stage = 0, phase = 0;
             bool alive = true;
-            detail::WgradUnit u;
-            for (uint32_t index = blockIdx.x; alive && detail::get_wgrad_unit(p, table, index, u); index += gridDim.x) {
+            while (alive && walk.next(p, schedule, u)) {
                 const bool second_box = u.col0 + 128 < p.k;
+                const uint32_t boxes = second_box ? 2 : 1;
                 for (uint32_t i = 0; i < u.count; ++i) {
                     const uint32_t kb = u.begin + i;
                     if (!detail::bounded_wait(empty + stage, phase ^ 1, abort_flag, p, 17)) {
@@ -353,7 +470,6 @@ __global__ void __launch_bounds__(384, 1)
                         break;
                     }
                     const bool scales = i == 0 || kb % 4 == 0;
-                    const uint32_t boxes = second_box ? 2 : 1;
                     ptx::mbar_arrive_expect_tx(full + stage, kMnBoxBytes * (1 + boxes) + (scales ? kScaleTileBytes * (1 + boxes) : 0u));
                     const int32_t token = static_cast<int32_t>((u.block0 + kb) * 128);
                     uint8_t* b = smem + T::kOffB + stage * T::kStageB;
@@ -379,13 +495,16 @@ __global__ void __launch_bounds__(384, 1)
             constexpr uint32_t idesc = make_instr_desc_mx_mn_major(128, T::kBlockFeatures);
             uint32_t stage = 0, phase = 0, sums_phase = 0, set = 0;
             bool alive = true;
-            detail::WgradUnit u;
-            for (uint32_t index = blockIdx.x; alive && detail::get_wgrad_unit(p, table, index, u); index += gridDim.x) {
-                if (u.count == 0) continue;
-                if (!detail::bounded_wait(sums_empty, sums_phase ^ 1, abort_flag, p, 18)) break;
-                ptx::tcgen05_fence_after_thread_sync();
+            while (alive && walk.next(p, schedule, u)) {
                 for (uint32_t i = 0; i < u.count; ++i) {
                     const uint32_t kb = u.begin + i;
+                    if (i % T::kChain == 0) {
+                        if (!detail::bounded_wait(sums_empty, sums_phase ^ 1, abort_flag, p, 18)) {
+                            alive = false;
+                            break;
+                        }
+                        sums_phase ^= 1;
+                    }
                     if (!detail::bounded_wait(full + stage, phase, abort_flag, p, 19)) {
                         alive = false;
                         break;
@@ -393,7 +512,7 @@ __global__ void __launch_bounds__(384, 1)
                     ptx::tcgen05_fence_after_thread_sync();
                     if (i == 0 || kb % 4 == 0) {
                         // Two sets in turn: the set that is written now was last used two quads ago, and a stage is loaded again only when
-                        // its products are complete, four k-blocks ago.
+                        // its products are complete, four k-blocks ago; a tile begins when the one in front is complete.
                         set ^= 1;
                         const uint32_t s = ptx::smem_u32(smem + T::kOffScales + stage * T::kStageScales);
 #pragma unroll
@@ -407,30 +526,35 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
                     for (uint32_t s = 0; s < 4; ++s)
                         ptx::umma_mxf8f6f4_ss(tmem, a + s * kMnKStep, b + s * kMnKStep, with_scale_byte(idesc, kb % 4), scale_a, scale_a + 4,
-                                              i != 0 || s != 0);
+                                              i % T::kChain != 0 || s != 0);
                     ptx::umma_commit(empty + stage);
+                    if (i % T::kChain == T::kChain - 1 || i + 1 == u.count) ptx::umma_commit(sums_full);
                     if (++stage == T::kStages) {
                         stage = 0;
                         phase ^= 1;
                     }
                 }
-                ptx::umma_commit(sums_full);
-                sums_phase ^= 1;
             }
         }
         __syncwarp();
     } else {
         // ---- sums -> dW ----
-        ptx::reg_alloc<232>();
+        ptx::reg_alloc<224>();  // 128 * 56 + 256 * 224 = 384 * 168, the launch's registers
         const uint32_t quarter = warp % 4, part = warp - 4, col0 = part / 4 * 128;
         const uint32_t box = ptx::smem_u32(smem + T::kOffStore + part * T::kBoxBytes);
         uint32_t sums_phase = 0;
-        detail::WgradUnit u;
-        for (uint32_t index = blockIdx.x; detail::get_wgrad_unit(p, table, index, u); index += gridDim.x) {
+        bool alive = true;
+        while (alive && walk.next(p, schedule, u)) {
             float acc[128];
-            if (u.count != 0) {
+#pragma unroll
+            for (uint32_t j = 0; j < 128; ++j) acc[j] = 0.0f;
+#pragma unroll 1
+            for (uint32_t i = 0; i < u.count; i += T::kChain) {
                 const bool ok = detail::bounded_wait(sums_full, sums_phase, abort_flag, p, 20);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (!__all_sync(0xffffffffu, ok)) {
+                    alive = false;
+                    break;
+                }
                 sums_phase ^= 1;
                 ptx::tcgen05_fence_after_thread_sync();
 #pragma unroll
@@ -438,38 +562,43 @@ __global__ void __launch_bounds__(384, 1)
                     uint32_t t[32];
                     ptx::tmem_ld_32x32b<32>(tmem + ((quarter * 32u) << 16) + col0 + c, t);
                     ptx::tmem_ld_wait<32>(t);
+                    if (c == 96) {
+                        ptx::tcgen05_fence_before_thread_sync();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(sums_empty);
+                    }
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; ++j) acc[c + j] = __uint_as_float(t[j]);
+                    for (uint32_t j = 0; j < 32; ++j) acc[c + j] += __uint_as_float(t[j]);
                 }
-                ptx::tcgen05_fence_before_thread_sync();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(sums_empty);
-                if (*abort_flag != 0) break;  // a wait ran out: the sums may be incomplete
-            } else {
-#pragma unroll
-                for (uint32_t j = 0; j < 128; ++j) acc[j] = 0.0f;
             }
-            if (p.slices > 1) {
-                float4* mine = p.partials + ((static_cast<uint64_t>(u.tile) * p.slices + u.slice) * 8 + part) * 1024 + lane;
+            if (!alive || *abort_flag != 0) break;  // a wait ran out: the sums may be incomplete
+            if (u.first_cta != u.last_cta) {
+                // Partial tiles meet in L2; who counts itself last adds them in the order of the tokens.  A CTA begins at most one tile
+                // that others end, and ends at most one that another began: a slot for each.
+                auto slot = [&](uint32_t cta) {
+                    return p.partials + (static_cast<uint64_t>(2 * cta + (cta == u.first_cta ? 1 : 0)) * 8 + part) * 1024 + lane;
+                };
+                float4* mine = slot(blockIdx.x);
 #pragma unroll
                 for (uint32_t j = 0; j < 32; ++j) __stcg(mine + j * 32, make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]));
                 __threadfence();
                 __syncwarp();
                 uint32_t before = 0;
-                if (lane == 0) before = atomicAdd(p.counters + u.tile * 8 + part, 1u);
-                if (__shfl_sync(0xffffffffu, before, 0) + 1 != p.slices) continue;
+                if (lane == 0) before = atomicAdd(p.counters + u.first_cta * 8 + part, 1u);
+                if (__shfl_sync(0xffffffffu, before, 0) != u.last_cta - u.first_cta) continue;
                 __threadfence();
-                const float4* from = p.partials + (static_cast<uint64_t>(u.tile) * p.slices * 8 + part) * 1024 + lane;
 #pragma unroll
                 for (uint32_t j = 0; j < 128; ++j) acc[j] = 0.0f;
-                for (uint32_t s = 0; s < p.slices; ++s, from += 8 * 1024) {
+#pragma unroll 1
+                for (uint32_t cta = u.first_cta; cta <= u.last_cta; ++cta) {
+                    const float4* from = slot(cta);
 #pragma unroll
                     for (uint32_t j = 0; j < 32; ++j) {
                         const float4 f = __ldcg(from + j * 32);
                         acc[4 * j] += f.x, acc[4 * j + 1] += f.y, acc[4 * j + 2] += f.z, acc[4 * j + 3] += f.w;
                     }
                 }
-            } else if (u.count == 0 && p.accumulate != 0) {
+            } else if (u.blocks == 0 && p.accumulate != 0) {
                 continue;
             }
             detail::store_wgrad_rows<out_t>(p, u, box, quarter * 32, col0, lane, acc);
@@ -507,27 +636,30 @@ struct WgradArgs {
 // What lies in the workspace, in this order, each on a 256-byte boundary.
 struct WgradWorkspace {
     size_t codes_n, codes_k, scales_n, scales_k, counters, partials, bytes;
-    uint32_t codes_ld_n, codes_ld_k, blocks, tiles, slices, num_counters;
+    uint32_t codes_ld_n, codes_ld_k, blocks, tiles, whole_tiles, ctas, num_counters;
 };
 
-// CTAs per tile: with fewer tiles than SMs the tokens of a tile are shared, as long as every CTA has four k-blocks.
-inline uint32_t choose_wgrad_slices(uint64_t tiles, uint32_t blocks_per_group, uint32_t num_sms) {
-    uint64_t slices = num_sms / tiles;
-    if (slices > blocks_per_group / 4) slices = blocks_per_group / 4;
-    return slices < 2 ? 1u : static_cast<uint32_t>(slices);
+// How many tiles are dealt out whole (see WgradSchedule): full waves, one less where more than half of another wave is left, because that
+// one would run nearly as long as a full one.
+inline uint32_t choose_whole_wgrad_tiles(uint32_t tiles, uint32_t ctas) {
+    const uint32_t waves = tiles / ctas, rest = tiles % ctas;
+    return (2 * rest > ctas && waves > 0 ? waves - 1 : waves) * ctas;
 }
 
-// `num_sms` only bounds the slices: the workspace for more SMs does for fewer.
 inline bool plan_wgrad_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t groups, bool grouped, uint32_t num_sms, WgradWorkspace& w) {
     w.blocks = max_token_blocks(rows, groups, grouped);
     w.codes_ld_n = align_up(n, 16u);
     w.codes_ld_k = align_up(k, 16u);
     const uint64_t tiles = static_cast<uint64_t>(ceil_div(n, 128u)) * ceil_div(k, WgradTile::kBlockFeatures) * groups;
-    if (tiles * 8 > 0x7fffffffull || static_cast<uint64_t>(w.blocks) * 128 > 0x7fffffffull || num_sms == 0) return false;
+    if (tiles > 0x7fffffffull || static_cast<uint64_t>(w.blocks) * 128 > 0x7fffffffull || num_sms == 0) return false;
     w.tiles = static_cast<uint32_t>(tiles);
-    w.slices = choose_wgrad_slices(tiles, ceil_div(rows, 128u * groups), num_sms);
+    // a CTA per tile, or per kMinCut k-blocks of one
+    const uint64_t useful = tiles * (1 + w.blocks / WgradTile::kMinCut);
+    w.ctas = useful < num_sms ? static_cast<uint32_t>(useful) : num_sms;
+    w.whole_tiles = choose_whole_wgrad_tiles(w.tiles, w.ctas);
+    const bool shared = w.whole_tiles != w.tiles && w.blocks >= WgradTile::kMinCut;  // tiles may be cut
     const uint64_t quads = max_token_quads(w.blocks, groups);
-    w.num_counters = w.slices > 1 ? w.tiles * 8 : 0;
+    w.num_counters = shared ? w.ctas * 8 : 0;
     size_t at = 0;
     auto take = [&at](size_t bytes) {
         const size_t here = at;
@@ -539,7 +671,7 @@ inline bool plan_wgrad_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t
     w.scales_n = take(quads * ceil_div(n, 128u) * kScaleTileBytes);
     w.scales_k = take(quads * ceil_div(k, 128u) * kScaleTileBytes);
     w.counters = take(w.num_counters * sizeof(uint32_t));
-    w.partials = take(w.slices > 1 ? tiles * w.slices * 128 * WgradTile::kBlockFeatures * sizeof(float) : 0);
+    w.partials = take(shared ? static_cast<size_t>(2) * w.ctas * 128 * WgradTile::kBlockFeatures * sizeof(float) : 0);
     w.bytes = at;
     return true;
 }
@@ -614,13 +746,14 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
     p.accumulate = a.accumulate;
     const uint32_t vec = 4, item = a.out_bf16 ? 2 : 4;  // four columns at a time
     p.vector_store = is_aligned(a.out, vec * item) && a.out_ld % vec == 0 && a.out_group % vec == 0 && a.k % vec == 0;
-    p.slices = w.slices;
+    p.tiles = w.tiles, p.whole_tiles = w.whole_tiles;
+    // A tile of 128 KB in fp32 leaves at 1/148 of the memory's rate in the time of about ten k-blocks.
+    p.store_cost = (a.out_bf16 ? 5u : 10u) * (a.accumulate ? 2u : 1u);
     p.partials = reinterpret_cast<float4*>(ws + w.partials);
     p.counters = reinterpret_cast<uint32_t*>(ws + w.counters);
     p.status = a.status;
     p.timeout_ns = a.timeout_ns;
-    const uint64_t units = static_cast<uint64_t>(w.tiles) * w.slices;
-    cfg.gridDim = dim3(static_cast<uint32_t>(units < static_cast<uint64_t>(a.num_sms) ? units : a.num_sms));
+    cfg.gridDim = dim3(w.ctas);
     cfg.blockDim = dim3(384);
     cfg.dynamicSmemBytes = WgradTile::kSmemSize;
     auto kernel = a.out_bf16 ? fp8_wgrad_kernel<__nv_bfloat16> : fp8_wgrad_kernel<float>;

@@ -71,10 +71,12 @@ __device__ __forceinline__ uint32_t first_sequence_behind(const BalanceParams& p
     return low;
 }
 
-// How the experts of a row lie over the lanes: kLanes lanes per row, kIter times kVec neighbouring experts each.
+// How the experts of a row lie over the lanes: kLanes lanes per row, kIter times kVec neighbouring experts each.  A warp has kRows rows
+// per group of lanes in flight, so that neither the loads nor the sums over the lanes are waited for one row at a time.
 template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
 struct BalanceRow {
-    static constexpr uint32_t kPerLane = kVec * kIter, kRowsPerWarp = 32 / kLanes;
+    static constexpr uint32_t kPerLane = kVec * kIter, kGroups = 32 / kLanes;
+    static constexpr uint32_t kRows = kPerLane <= 8 ? 4 : kPerLane <= 16 ? 2 : 1, kRowsPerWarp = kGroups * kRows;
 
     __device__ __forceinline__ static uint32_t column(uint32_t lane, uint32_t c) {
         return (c / kVec * kLanes + lane % kLanes) * kVec + c % kVec;
@@ -87,9 +89,8 @@ struct BalanceRow {
             if constexpr (kVec == 1) {
                 z[i] = there && col < experts ? static_cast<float>(row[col]) : -INFINITY;
             } else {
-                uint4 v;
                 const uint32_t nothing = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
-                v = make_uint4(nothing, nothing, nothing, nothing);
+                uint4 v = make_uint4(nothing, nothing, nothing, nothing);
                 if (there && col < experts) v = *reinterpret_cast<const uint4*>(row + col);
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -104,6 +105,7 @@ struct BalanceRow {
             }
         }
     }
+    // The gradient is not read again here: it leaves L2 before the logits do.
     __device__ __forceinline__ static void store(T* row, uint32_t experts, uint32_t lane, const float (&z)[kPerLane]) {
 #pragma unroll
         for (uint32_t i = 0; i < kIter; ++i) {
@@ -112,7 +114,7 @@ struct BalanceRow {
             if constexpr (kVec == 1) {
                 row[col] = static_cast<T>(z[i]);
             } else if constexpr (sizeof(T) == 4) {
-                *reinterpret_cast<float4*>(row + col) = make_float4(z[i * 4], z[i * 4 + 1], z[i * 4 + 2], z[i * 4 + 3]);
+                __stcs(reinterpret_cast<float4*>(row + col), make_float4(z[i * 4], z[i * 4 + 1], z[i * 4 + 2], z[i * 4 + 3]));
             } else {
                 uint32_t w[4];
 #pragma unroll
@@ -120,7 +122,7 @@ struct BalanceRow {
                     const __nv_bfloat162 t = __floats2bfloat162_rn(z[i * 8 + 2 * j], z[i * 8 + 2 * j + 1]);
                     w[j] = *reinterpret_cast<const uint32_t*>(&t);
                 }
-                *reinterpret_cast<uint4*>(row + col) = make_uint4(w[0], w[1], w[2], w[3]);
+                __stcs(reinterpret_cast<uint4*>(row + col), make_uint4(w[0], w[1], w[2], w[3]));
             }
         }
     }
@@ -134,13 +136,123 @@ struct BalanceRow {
         for (uint32_t off = kLanes / 2; off >= 1; off /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
         return v;
     }
-    // z -> scores that add up to 1 / inverse; `shift` is the largest logit (softmax).  A row of nothing but -inf has zeros.
+    // z -> scores before they are divided by their sum; `shift` is the largest logit (softmax).
     __device__ __forceinline__ static void scores(bool sigmoid, float (&z)[kPerLane], float shift) {
+        if (sigmoid) {
 #pragma unroll
-        for (uint32_t c = 0; c < kPerLane; ++c)
-            z[c] = sigmoid ? __fdividef(1.0f, 1.0f + __expf(-z[c])) : __expf(z[c] - shift);
+            for (uint32_t c = 0; c < kPerLane; ++c) z[c] = __fdividef(1.0f, 1.0f + __expf(-z[c]));
+        } else {
+#pragma unroll
+            for (uint32_t c = 0; c < kPerLane; ++c) z[c] = __expf(z[c] - shift);
+        }
+    }
+
+    // Adds the probabilities of tokens [begin, end) that the warp has its turn for, and counts those that count.  rows[token]: what
+    // their gradient needs, if there is to be one.
+    __device__ __forceinline__ static void add(const BalanceParams& p, uint32_t begin, uint32_t end, uint32_t warp, uint32_t warps, uint32_t lane,
+                                               float2* rows, float (&sums)[kPerLane], int& counted) {
+        const T* logits = static_cast<const T*>(p.logits);
+        for (uint32_t base = begin + warp * kRowsPerWarp; base < end; base += warps * kRowsPerWarp) {
+            float z[kRows][kPerLane], shift[kRows], total[kRows];
+            bool counts[kRows];
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                const uint32_t token = base + r * kGroups + lane / kLanes;
+                counts[r] = token < end && (p.mask == nullptr || p.mask[token] != 0);
+                load(logits + static_cast<uint64_t>(token) * p.logits_ld, counts[r], p.experts, lane, z[r]);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                shift[r] = 0.0f;
+                if (p.sigmoid == 0) {
+                    shift[r] = z[r][0];
+#pragma unroll
+                    for (uint32_t c = 1; c < kPerLane; ++c) shift[r] = fmaxf(shift[r], z[r][c]);
+                    shift[r] = largest(shift[r]);
+                    if (shift[r] == -INFINITY) shift[r] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                scores(p.sigmoid != 0, z[r], shift[r]);
+                total[r] = 0.0f;
+#pragma unroll
+                for (uint32_t c = 0; c < kPerLane; ++c) total[r] += z[r][c];
+                total[r] = sum(total[r]);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                const float inverse = total[r] == 0.0f ? 0.0f : 1.0f / total[r];  // a row of nothing but -inf has zeros
+#pragma unroll
+                for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = fmaf(z[r][c], inverse, sums[c]);
+                if (lane % kLanes == 0 && counts[r]) {
+                    if (rows != nullptr) rows[base + r * kGroups + lane / kLanes] = make_float2(shift[r], inverse);
+                    ++counted;
+                }
+            }
+        }
+    }
+
+    // The gradient of tokens [at, end) that the warp has its turn for; those in front of `begin` and those that do not count have zeros.
+    __device__ __forceinline__ static void grad(const BalanceParams& p, uint32_t at, uint32_t begin, uint32_t end, uint32_t warp, uint32_t warps,
+                                                uint32_t lane, const float2* rows, const float (&weights)[kPerLane]) {
+        const T* logits = static_cast<const T*>(p.logits);
+        T* out = static_cast<T*>(p.grad);
+        for (uint32_t base = at + warp * kRowsPerWarp; base < end; base += warps * kRowsPerWarp) {
+            float z[kRows][kPerLane], inner[kRows];
+            float2 row[kRows];
+            bool counts[kRows];
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                const uint32_t token = base + r * kGroups + lane / kLanes;
+                counts[r] = token >= begin && token < end && (p.mask == nullptr || p.mask[token] != 0);
+                load(logits + static_cast<uint64_t>(token) * p.logits_ld, counts[r], p.experts, lane, z[r]);
+                row[r] = counts[r] ? rows[token] : make_float2(0.0f, 0.0f);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                scores(p.sigmoid != 0, z[r], row[r].x);
+                inner[r] = 0.0f;
+#pragma unroll
+                for (uint32_t c = 0; c < kPerLane; ++c) inner[r] = fmaf(z[r][c], weights[c], inner[r]);
+                inner[r] = sum(inner[r]);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                const uint32_t token = base + r * kGroups + lane / kLanes;
+                inner[r] *= row[r].y;
+#pragma unroll
+                for (uint32_t c = 0; c < kPerLane; ++c) {
+                    const float slope = p.sigmoid != 0 ? z[r][c] * (1.0f - z[r][c]) : z[r][c];
+                    z[r][c] = counts[r] ? slope * row[r].y * (weights[c] - inner[r]) : 0.0f;
+                }
+                if (token < end) store(out + static_cast<uint64_t>(token) * p.grad_ld, p.experts, lane, z[r]);
+            }
+        }
     }
 };
+
+// Adds the selections of tokens [begin, end) that count to s_counts.
+__device__ __forceinline__ void count_selections(const BalanceParams& p, uint32_t begin, uint32_t end, uint32_t thread, uint32_t threads,
+                                                 int* s_counts) {
+    const uint64_t first = static_cast<uint64_t>(begin) * p.top, last = static_cast<uint64_t>(end) * p.top;
+    for (uint64_t i = first + thread; i < last; i += threads) {
+        if (p.mask != nullptr) {
+            const uint32_t token = last <= 0xFFFFFFFFu ? static_cast<uint32_t>(i) / p.top : static_cast<uint32_t>(i / p.top);
+            if (p.mask[token] == 0) continue;
+        }
+        const long long id = p.ids_64 != 0 ? static_cast<const long long*>(p.ids)[i] : static_cast<const int*>(p.ids)[i];
+        if (id >= 0 && id < static_cast<long long>(p.experts)) atomicAdd(&s_counts[id], 1);
+    }
+}
+
+// a of an expert with `count` selections in a sequence of `tokens` that count.
+__device__ __forceinline__ float balance_weight(const BalanceParams& p, int count, int tokens) {
+    const float n = static_cast<float>(tokens);
+    return tokens <= 0 ? 0.0f
+                       : p.coef / static_cast<float>(p.sequences) * (static_cast<float>(p.experts) / (static_cast<float>(p.top) * n)) *
+                             (static_cast<float>(count) / n);
+}
 
 }  // namespace detail
 
@@ -152,9 +264,9 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_sums_kernel(const Bal
     __shared__ int s_counts[kMaxBalanceExperts];
     __shared__ int s_tokens;
     ptx::grid_dependency_wait();
+    ptx::grid_dependency_launch_dependents();  // the next launch waits for the end of this one before it reads anything
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t strip = blockIdx.x, first = strip * p.strip_tokens, last = min(first + p.strip_tokens, p.tokens);
-    const T* logits = static_cast<const T*>(p.logits);
     for (uint32_t s = detail::first_sequence_behind(p, first); s < p.sequences; ++s) {
         uint32_t begin, end;
         detail::sequence_range(p, s, begin, end);
@@ -164,46 +276,12 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_sums_kernel(const Bal
         for (uint32_t e = threadIdx.x; e < p.experts; e += kBalanceThreads) s_counts[e] = 0;
         if (threadIdx.x == 0) s_tokens = 0;
         __syncthreads();
-        // selections
-        const uint64_t pairs = static_cast<uint64_t>(end - begin) * p.top;
-        for (uint64_t i = threadIdx.x; i < pairs; i += kBalanceThreads) {
-            const uint32_t token = begin + static_cast<uint32_t>(i / p.top);
-            if (p.mask != nullptr && p.mask[token] == 0) continue;
-            const uint64_t at = static_cast<uint64_t>(begin) * p.top + i;
-            const long long id = p.ids_64 != 0 ? static_cast<const long long*>(p.ids)[at] : static_cast<const int*>(p.ids)[at];
-            if (id >= 0 && id < static_cast<long long>(p.experts)) atomicAdd(&s_counts[id], 1);
-        }
-        // probabilities
+        detail::count_selections(p, begin, end, threadIdx.x, kBalanceThreads, s_counts);
         float sums[kPerLane];
 #pragma unroll
         for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = 0.0f;
         int counted = 0;
-        for (uint32_t base = begin + warp * Row::kRowsPerWarp; base < end; base += kBalanceWarps * Row::kRowsPerWarp) {
-            const uint32_t token = base + lane / kLanes;
-            const bool counts = token < end && (p.mask == nullptr || p.mask[token] != 0);
-            float z[kPerLane];
-            Row::load(logits + static_cast<uint64_t>(token) * p.logits_ld, counts, p.experts, lane, z);
-            float shift = 0.0f;
-            if (p.sigmoid == 0) {
-                shift = z[0];
-#pragma unroll
-                for (uint32_t c = 1; c < kPerLane; ++c) shift = fmaxf(shift, z[c]);
-                shift = Row::largest(shift);
-                if (shift == -INFINITY) shift = 0.0f;
-            }
-            Row::scores(p.sigmoid != 0, z, shift);
-            float total = 0.0f;
-#pragma unroll
-            for (uint32_t c = 0; c < kPerLane; ++c) total += z[c];
-            total = Row::sum(total);
-            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-            for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = fmaf(z[c], inverse, sums[c]);
-            if (lane % kLanes == 0 && counts) {
-                if (p.grad != nullptr) p.rows[token] = make_float2(shift, inverse);
-                ++counted;
-            }
-        }
+        Row::add(p, begin, end, warp, kBalanceWarps, lane, p.grad != nullptr ? p.rows : nullptr, sums, counted);
         if (counted != 0) atomicAdd(&s_tokens, counted);
 #pragma unroll
         for (uint32_t c = 0; c < kPerLane; ++c) {
@@ -226,19 +304,22 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_sums_kernel(const Bal
     }
 }
 
-// One CTA: 32 experts of one sequence; eight threads share an expert's slots.
-__global__ void __launch_bounds__(kBalanceThreads) balance_weights_kernel(const BalanceParams p) {
-    __shared__ float s_sum[8][32];
-    __shared__ int s_count[8][32], s_tokens[8];
+// One CTA: 32 experts of one sequence; 32 warps share an expert's slots.
+constexpr uint32_t kBalanceWeightWarps = 32;
+__global__ void __launch_bounds__(kBalanceWeightWarps * 32) balance_weights_kernel(const BalanceParams p) {
+    __shared__ float s_sum[kBalanceWeightWarps][32];
+    __shared__ int s_count[kBalanceWeightWarps][32], s_tokens[kBalanceWeightWarps];
     ptx::grid_dependency_wait();
-    const uint32_t s = blockIdx.y, e = blockIdx.x * 32 + threadIdx.x % 32, part = threadIdx.x / 32;
+    ptx::grid_dependency_launch_dependents();
+    const uint32_t s = blockIdx.y, lane = threadIdx.x % 32, e = blockIdx.x * 32 + lane, part = threadIdx.x / 32;
     uint32_t begin, end;
     detail::sequence_range(p, s, begin, end);
     float sum = 0.0f;
     int count = 0, tokens = 0;
     if (begin < end) {
         const uint64_t from = begin / p.strip_tokens + s, to = (end - 1) / p.strip_tokens + s;
-        for (uint64_t slot = from + part; slot <= to; slot += 8) {
+#pragma unroll 4
+        for (uint64_t slot = from + part; slot <= to; slot += kBalanceWeightWarps) {
             if (e < p.experts) {
                 sum += p.slot_sums[slot * p.experts + e];
                 count += p.slot_counts[slot * p.experts + e];
@@ -246,27 +327,24 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_weights_kernel(const 
             tokens += p.slot_tokens[slot];
         }
     }
-    s_sum[part][threadIdx.x % 32] = sum;
-    s_count[part][threadIdx.x % 32] = count;
-    if (threadIdx.x % 32 == 0) s_tokens[part] = tokens;
+    s_sum[part][lane] = sum;
+    s_count[part][lane] = count;
+    if (lane == 0) s_tokens[part] = tokens;
     __syncthreads();
     if (part != 0) return;
     sum = 0.0f, count = 0, tokens = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) sum += s_sum[i][threadIdx.x], count += s_count[i][threadIdx.x], tokens += s_tokens[i];
-    const float n = static_cast<float>(tokens);
+    for (uint32_t i = 0; i < kBalanceWeightWarps; ++i) sum += s_sum[i][lane], count += s_count[i][lane], tokens += s_tokens[i];
     float weight = 0.0f;
     if (e < p.experts) {
-        if (tokens > 0)
-            weight = p.coef / static_cast<float>(p.sequences) * (static_cast<float>(p.experts) / (static_cast<float>(p.top) * n)) *
-                     (static_cast<float>(count) / n);
+        weight = detail::balance_weight(p, count, tokens);
         p.weights[static_cast<uint64_t>(s) * p.experts + e] = weight;
         p.counts[static_cast<uint64_t>(s) * p.experts + e] = count;
     }
     float loss = weight * sum;
 #pragma unroll
     for (uint32_t off = 16; off >= 1; off /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, off);
-    if (threadIdx.x == 0) p.losses[s * gridDim.x + blockIdx.x] = loss;
+    if (lane == 0) p.losses[s * gridDim.x + blockIdx.x] = loss;
 }
 
 // Strips from the last to the first: what the first launch read last is what L2 still holds.
@@ -285,8 +363,6 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_grad_kernel(const Bal
     }
     if (p.grad == nullptr) return;
     const uint32_t strip = gridDim.x - 1 - blockIdx.x, first = strip * p.strip_tokens, last = min(first + p.strip_tokens, p.tokens);
-    const T* logits = static_cast<const T*>(p.logits);
-    T* grad = static_cast<T*>(p.grad);
     float weights[kPerLane];
     uint32_t at = first;  // tokens below have their gradient
     for (uint32_t s = detail::first_sequence_behind(p, first); at < last; ++s) {
@@ -301,24 +377,7 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_grad_kernel(const Bal
                 weights[c] = col < p.experts ? p.weights[static_cast<uint64_t>(s) * p.experts + col] : 0.0f;
             }
         }
-        for (uint32_t base = at + warp * Row::kRowsPerWarp; base < end; base += kBalanceWarps * Row::kRowsPerWarp) {
-            const uint32_t token = base + lane / kLanes;
-            const bool counts = token >= begin && token < end && (p.mask == nullptr || p.mask[token] != 0);
-            float z[kPerLane];
-            Row::load(logits + static_cast<uint64_t>(token) * p.logits_ld, counts, p.experts, lane, z);
-            const float2 row = counts ? p.rows[token] : make_float2(0.0f, 0.0f);
-            Row::scores(p.sigmoid != 0, z, row.x);
-            float inner = 0.0f;
-#pragma unroll
-            for (uint32_t c = 0; c < kPerLane; ++c) inner = fmaf(z[c], weights[c], inner);
-            inner = Row::sum(inner) * row.y;
-#pragma unroll
-            for (uint32_t c = 0; c < kPerLane; ++c) {
-                const float slope = p.sigmoid != 0 ? z[c] * (1.0f - z[c]) : z[c];
-                z[c] = counts ? slope * row.y * (weights[c] - inner) : 0.0f;
-            }
-            if (token < end) Row::store(grad + static_cast<uint64_t>(token) * p.grad_ld, p.experts, lane, z);
-        }
+        Row::grad(p, at, begin, end, warp, kBalanceWarps, lane, p.rows, weights);
         at = end;
     }
 }
@@ -333,8 +392,11 @@ struct BalanceWorkspace {
 
 inline BalanceWorkspace plan_balance_workspace(uint32_t tokens, uint32_t experts, uint32_t sequences, bool with_grad, uint32_t num_sms) {
     BalanceWorkspace w;
+#ifndef BS
+#define BS 3
+#endif
     // two CTAs per SM, at least four tokens per warp
-    w.strip_tokens = ceil_div(tokens, 2 * num_sms);
+    w.strip_tokens = ceil_div(tokens, BS * num_sms);
     if (w.strip_tokens < 4 * kBalanceWarps) w.strip_tokens = 4 * kBalanceWarps;
     w.strips = ceil_div(tokens, w.strip_tokens);
     if (w.strips == 0) w.strips = 1;
@@ -371,8 +433,10 @@ inline int launch_balance_as(const BalanceParams& p, cudaStream_t stream) {
     cfg.dynamicSmemBytes = 0;
     const uint32_t parts = ceil_div(p.experts, 32u);
     cfg.gridDim = dim3(parts, p.sequences);
+    cfg.blockDim = dim3(kBalanceWeightWarps * 32);
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, balance_weights_kernel, p);
     cfg.gridDim = dim3(p.grad != nullptr ? p.strips : 1u);
+    cfg.blockDim = dim3(kBalanceThreads);
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, balance_grad_kernel<T, kVec, kLanes, kIter>, p, parts * p.sequences);
     if (e != cudaSuccess) {
         cudaGetLastError();

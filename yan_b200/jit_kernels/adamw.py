@@ -50,6 +50,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     grad_scale: fp32 tensor of one element on the device (a clipping factor, say), read when the kernel runs.
     copies: bf16 tensors that receive the new parameters, e.g. what per_block_cast_to_fp8 quantizes for the next forward pass.
     lr, step and the other numbers become part of a captured CUDA graph."""
+    rc = _lib.fast().adamw(params, grads, exp_avgs, exp_avg_sqs, weight_decay, copies, grad_scale, lr, beta1, beta2, eps, step)
+    if rc != -1:  # -1: not an ordinary call, left to the checks below
+        return _lib.check("yan_b200_adamw_step", rc)
     count = len(params)
     assert len(grads) == count and len(exp_avgs) == count and len(exp_avg_sqs) == count and (copies is None or len(copies) == count)
     decays = [float(weight_decay)] * count if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
@@ -57,7 +60,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if count == 0:
         return
     device, param_dtype, grad_dtype = params[0].device, params[0].dtype, grads[0].dtype
-    assert params[0].is_cuda and param_dtype in _DTYPES and grad_dtype in _DTYPES, "params and grads are fp32 or bf16 on the GPU"
+    assert params[0].is_cuda and device.index == torch.cuda.current_device()
+    assert param_dtype in _DTYPES and grad_dtype in _DTYPES, "params and grads are fp32 or bf16 on the GPU"
     eight_bit = not isinstance(exp_avgs[0], torch.Tensor)
     if grad_scale is not None:
         assert grad_scale.device == device and grad_scale.dtype == torch.float32 and grad_scale.numel() == 1
@@ -73,5 +77,6 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             c = copies[i]
             assert c.dtype == torch.bfloat16 and c.device == device and c.is_contiguous() and c.numel() == p.numel()
             row.copy = c.data_ptr()
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])  # autograd notices that they change
     _lib.call("yan_b200_adamw_step", table, count, _DTYPES[param_dtype], _DTYPES[grad_dtype], 8 if eight_bit else 32, lr, beta1, beta2, eps,
               step, grad_scale.data_ptr() if grad_scale is not None else None, _lib.current_stream_ptr())

@@ -7,6 +7,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
+from . import utils as _utils
 from .utils import get_num_sms
 
 MAX_EXPERTS = 1024
@@ -36,7 +37,14 @@ def moe_balance_loss(logits: torch.Tensor, expert_ids: torch.Tensor, *, coef: fl
     [0, E) selects nothing (a dropped token).  token_mask [T] bool: tokens that count; the logits of the others are not read and their
     gradient is zero.  cu_seqlens int32 [S + 1], ascending, on the device: sequence s is tokens [cu_seqlens[s], cu_seqlens[s + 1]); without it
     all tokens are one sequence.  A sequence without tokens adds nothing.  loss is an fp32 tensor without dimensions."""
-    assert logits.is_cuda and logits.dim() == 2 and logits.dtype in _DTYPES, "logits are [T, E] in fp32 or bf16"
+    if with_grad and grad is None and workspace is None and _utils._num_sms is not None and score in _SCORES:
+        result = _lib.fast().balance(logits, expert_ids, token_mask, cu_seqlens, coef, _SCORES[score], _utils._num_sms)
+        if type(result) is tuple:
+            return result
+        if result != -1:  # -1: not an ordinary call, left to the checks below
+            _lib.check("yan_b200_moe_balance_loss", result)
+    assert logits.is_cuda and logits.device.index == torch.cuda.current_device()
+    assert logits.dim() == 2 and logits.dtype in _DTYPES, "logits are [T, E] in fp32 or bf16"
     t, e = logits.shape
     assert 0 < e <= MAX_EXPERTS and (e == 1 or logits.stride(1) == 1)
     assert expert_ids.device == logits.device and expert_ids.dim() == 2 and expert_ids.shape[0] == t and expert_ids.shape[1] > 0

@@ -10,6 +10,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
+from . import utils as _utils
 from .utils import get_num_sms
 
 MAX_GROUPS = 512
@@ -17,7 +18,7 @@ _OUT_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
 def _check_operands(dy: torch.Tensor, x: torch.Tensor) -> None:
-    assert dy.is_cuda and x.is_cuda and dy.device == x.device
+    assert dy.is_cuda and x.is_cuda and dy.device == x.device and dy.device.index == torch.cuda.current_device()
     assert dy.dtype == torch.bfloat16 and x.dtype == torch.bfloat16 and dy.dim() == 2 and x.dim() == 2
     assert dy.shape[0] == x.shape[0], "dy and x have a row per token"
     assert dy.shape[1] > 0 and x.shape[1] > 0
@@ -58,6 +59,11 @@ def fp8_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, out: Optional[torch.Tens
     Any number of tokens (none included) and of features and any row strides; rows on 32-byte boundaries with multiples of 16
     features are the fast case.  The scratch comes from torch's allocator unless a `workspace` of
     fp8_linear_wgrad_workspace_bytes(M, N, K) bytes is given."""
+    if out is not None and _utils._num_sms is not None:
+        rc = _lib.fast().wgrad(dy, x, out, accumulate, workspace, _utils._num_sms, None, None)
+        if rc != -1:  # -1: not an ordinary call, left to the checks below
+            _lib.check("yan_b200_fp8_linear_wgrad", rc)
+            return out
     _check_operands(dy, x)
     m, n, k = dy.shape[0], dy.shape[1], x.shape[1]
     if out is None:
@@ -80,6 +86,11 @@ def k_grouped_fp8_linear_wgrad(dy: torch.Tensor, x: torch.Tensor, group_starts: 
     of m_grouped_gemm_fp8_fp8_bf16_nt_contiguous, whose starts are multiples of 128, or rows packed without gaps.  Groups do not
     overlap; rows outside of every group are not read.  A group without rows gives zeros, or leaves its part of `out` as it is
     with accumulate=True.  Otherwise like fp8_linear_wgrad."""
+    if out is not None and _utils._num_sms is not None:
+        rc = _lib.fast().wgrad(dy, x, out, accumulate, workspace, _utils._num_sms, group_starts, group_sizes)
+        if rc != -1:
+            _lib.check("yan_b200_k_grouped_fp8_linear_wgrad", rc)
+            return out
     _check_operands(dy, x)
     m, n, k, g = dy.shape[0], dy.shape[1], x.shape[1], group_sizes.numel()
     assert 0 < g <= MAX_GROUPS
