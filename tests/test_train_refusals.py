@@ -30,10 +30,10 @@ def test_wgrad_workspace():
     size = _lib.lib().yan_b200_fp8_linear_wgrad_workspace_bytes
     assert _wgrad(ws_bytes=size(64, 32, 48, 0, 148) - 1) == SMALL
     assert size(-1, 32, 48, 0, 148) == 0 and size(64, 0, 48, 0, 148) == 0 and size(64, 32, 48, 0, 0) == 0
-    # codes of 128 tokens, a scale tile per operand, and nothing shared between CTAs
-    assert size(64, 32, 48, 0, 148) == 128 * 32 + 128 * 48 + 2 * 512
+    # codes of 128 tokens, scale tiles (128 features of dy; up to 256 of x), and nothing shared between CTAs
+    assert size(64, 32, 48, 0, 148) == 128 * 32 + 128 * 48 + 512 + 1024
     # groups can begin anywhere: a block of tokens more for each
-    assert size(64, 32, 48, 4, 148) == 4 * 128 * (32 + 48) + 5 * 2 * 512
+    assert size(64, 32, 48, 4, 148) == 4 * 128 * (32 + 48) + 5 * (512 + 1024)
 
 
 @pytest.mark.parametrize("change", [dict(starts=None), dict(sizes=None), dict(groups=0), dict(groups=513)])

@@ -4,8 +4,8 @@
 //
 //   1. block_cast_tokens_kernel: both bf16 operands -> e4m3 codes, in the order they have, with one power of two per feature and block
 //      of 128 tokens, e the smallest integer with amax <= 448 * 2^e.  A block that ends a group is filled up with zeros.
-//   2. fp8_wgrad_kernel: persistent, warp-specialised tcgen05 products of 128 x 256 tiles of dW, summed over the tokens in tensor memory.
-//      The tensor core transposes the token-major operands and multiplies the scales in, so that nothing has to be promoted.
+//   2. fp8_wgrad_kernel: persistent, warp-specialised tcgen05 products of tiles of dW by pairs of CTAs, summed over the tokens in tensor
+//      memory.  The tensor core transposes the token-major operands and multiplies the scales in, so that nothing has to be promoted.
 
 #include <cstdint>
 #include <cuda.h>
@@ -29,7 +29,8 @@ struct CastTokensOperand {
     uint32_t wide = 0;         // rows start on 32-byte boundaries and have whole groups of 16 columns
     uint8_t* codes = nullptr;  // [blocks * 128][codes_ld], codes_ld a multiple of 16
     uint32_t codes_ld = 0;
-    uint8_t* scales = nullptr;  // [quads][ceil(cols / 128)] scale tiles
+    uint8_t* scales = nullptr;  // [quads][ceil(cols / scale_cols)][ceil(scale_cols / 128)] scale tiles
+    uint32_t scale_cols = 128;  // columns of one tile of products
 };
 
 struct CastTokensParams {
@@ -129,8 +130,10 @@ __global__ void __launch_bounds__(256) block_cast_tokens_kernel(const CastTokens
         for (uint32_t w = 0; w < 8; ++w) amax = max(amax, static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(s_max[w])[thread]));
         const uint32_t scale = detail::scale_byte_of_amax(amax);
         s_scale[thread] = static_cast<uint8_t>(scale);
-        op.scales[(static_cast<uint64_t>(quad) * p.column_tiles[second] + tile) * kScaleTileBytes + scale_tile_offset(thread, byte)] =
-            static_cast<uint8_t>(scale);
+        const uint32_t c = tile * 128 + thread, in_tile = c % op.scale_cols;
+        if (c < op.cols)
+            op.scales[((static_cast<uint64_t>(quad) * ceil_div(op.cols, op.scale_cols) + c / op.scale_cols) * ceil_div(op.scale_cols, 128u) +
+                       in_tile / 128) * kScaleTileBytes + scale_tile_offset(in_tile % 128, byte)] = static_cast<uint8_t>(scale);
     }
     __syncthreads();
     if (col >= op.codes_ld) return;
@@ -155,25 +158,23 @@ struct WgradParams {
     TokenGroups groups;
     uint32_t max_blocks = 0;
     uint32_t n = 0, k = 0;                // sides of dW
-    const uint8_t* scales_n = nullptr;    // of dy: [quads][ceil(n / 128)] scale tiles
-    const uint8_t* scales_k = nullptr;    // of x
     void* out = nullptr;                  // [groups][n][out_ld]
     uint64_t out_ld = 0, out_group = 0;   // elements
     uint32_t accumulate = 0;
     uint32_t vector_store = 0;            // rows of dW allow four elements at a time
     uint32_t tiles = 0, whole_tiles = 0;  // all of them; those that are dealt out one by one (see WgradSchedule)
     uint32_t store_cost = 0;              // k-blocks that take as long as storing a tile
-    float4* partials = nullptr;           // [2 * CTAs][8 warps][32][32 lanes]
-    uint32_t* counters = nullptr;         // [CTAs][8 warps], zero
+    float4* partials = nullptr;           // [2 * pairs][2 CTAs][8 warps][columns of a warp / 4][32 lanes]
+    uint32_t* counters = nullptr;         // [pairs][2 CTAs][8 warps], zero
     int* status = nullptr;
     unsigned long long timeout_ns = 0;
 };
 
-// Who computes what.  Tiles are numbered group by group, within a group in bands of 16 tile rows, so that CTAs at work at the same time
-// share what they read.  The first whole_tiles of them, a multiple of the CTAs, are dealt out in turn.  The rest, less than two waves,
+// Who computes what.  Tiles are numbered group by group, within a group in bands of eight tile rows, so that pairs at work at the same time
+// share what they read.  The first whole_tiles of them, a multiple of the pairs, are dealt out in turn.  The rest, less than two waves,
 // is shared evenly: laid end to end, a tile as long as its k-blocks or as its store takes, whichever is more, and cut into one
-// stretch per CTA.  A cut through the k-blocks of a tile goes to a multiple of four of them; tiles of fewer than kMinCut go whole to
-// the CTA in whose stretch they begin.
+// stretch per pair.  A cut through the k-blocks of a tile goes to a multiple of four of them; tiles of fewer than kMinCut go whole to
+// the pair in whose stretch they begin.
 struct WgradSchedule {
     TokenBlockTable blocks;
     uint64_t length[kMaxTokenGroups + 1];  // of all tiles in front of a group
@@ -181,38 +182,48 @@ struct WgradSchedule {
     uint32_t stretches;
 };
 
+// A pair of CTAs computes 256 x kCols of dW at a time, each CTA 128 rows of it: per 128 tokens it loads 128 rows of A and kCols / 2 columns of
+// B, where a CTA by itself would load all kCols.  What bounds long sums is the power limit (1.28 GHz at N=28672 K=8192), so that bytes
+// moved per product count more than cycles: quantization and products together there 1.74 ms with pairs and 256 columns, 1.81 with 192
+// (whose two accumulators lie side by side, so that nothing ever waits for sums to be read), 2.12 with 224, 1.95 with single CTAs of
+// 128 x 256.
+constexpr uint32_t kWgradRows = 256;
+constexpr uint32_t kWgradMinCut = 8, kWgradMinStretch = 8;
+
+template <uint32_t kCols>
 struct WgradTile {
-    static constexpr uint32_t kBlockFeatures = 256;  // columns of a tile (features of x); its rows are 128 features of dy
-    static constexpr uint32_t kStages = 4;
-    // k-blocks that are summed in tensor memory before the sums move to registers.  An addition there rounds towards zero (8192 tokens of
-    // uneven size, relative error: 1.3e-6 in one chain).
-#ifndef YAN_WGRAD_CHAIN
-#define YAN_WGRAD_CHAIN 32
-#endif
-    static constexpr uint32_t kChain = YAN_WGRAD_CHAIN;
-    static constexpr uint32_t kMinCut = 8, kMinStretch = 8;
-    static constexpr uint32_t kStageA = kMnBoxBytes, kStageB = 2 * kMnBoxBytes;
-    static constexpr uint32_t kScaleTiles = 1 + kBlockFeatures / 128;
+    static constexpr uint32_t kStages = 6;
+    // k-blocks that are summed in tensor memory before the sums move to registers.  An addition there rounds towards zero: 8192 tokens of
+    // uneven size, relative error 1.3e-6 in one chain of 64 k-blocks, 5e-7 in chains of 32, 2.2e-7 in chains of 16.  Where the
+    // accumulators share columns the products wait at the end of a chain: N=28672 K=8192, 8192 tokens, 1.72, 1.74 and 1.85 ms.
+    static constexpr uint32_t kChain = kCols <= 192 ? 16 : 32;
+    static constexpr uint32_t kStageA = kMnBoxBytes, kStageB = kMnBoxBytes;
+    static constexpr uint32_t kScaleTiles = 1 + ceil_div(kCols, 128u);
     static constexpr uint32_t kStageScales = kScaleTiles * kScaleTileBytes;
     static constexpr uint32_t kOffA = 0, kOffB = kOffA + kStages * kStageA, kOffScales = kOffB + kStages * kStageB;
     static constexpr uint32_t kBoxRowBytes = 64, kBoxBytes = 32 * kBoxRowBytes;  // output staging, one box per warp
     static constexpr uint32_t kOffStore = kOffScales + kStages * kStageScales;
     static constexpr uint32_t kOffSchedule = kOffStore + 8 * kBoxBytes;
     static constexpr uint32_t kOffBarriers = align_up(kOffSchedule + static_cast<uint32_t>(sizeof(WgradSchedule)), 8u);
-    static constexpr uint32_t kNumBarriers = 2 * kStages + 2;
+    static constexpr uint32_t kNumBarriers = 2 * kStages + 6;
     static constexpr uint32_t kOffTmemSlot = kOffBarriers + kNumBarriers * 8, kOffAbort = kOffTmemSlot + 4;
     static constexpr uint32_t kSmemSize = kOffAbort + 4 + 1024;
-    // tensor memory: the sums, then two sets of scales
-    static constexpr uint32_t kTmemScales = kBlockFeatures, kTmemScaleSet = kScaleTiles * 4, kTmemCols = 512;
-    static_assert(kTmemScales + 2 * kTmemScaleSet <= kTmemCols);
+    static constexpr uint32_t kWarpCols = kCols / 2;  // columns of a warp that reads sums
+    // tensor memory: two accumulators, then three sets of scales.  Where they do not fit side by side the accumulators share kShared
+    // columns, the last of the first and the first of the second, which are read before the others and handed on by themselves.
+    static constexpr uint32_t kTmemCols = 512, kTmemScaleSet = kScaleTiles * 4;
+    static constexpr uint32_t kShared = 2 * kCols + 3 * kTmemScaleSet <= kTmemCols ? 0 : align_up(2 * kCols + 3 * kTmemScaleSet - kTmemCols, 16u);
+    static constexpr uint32_t kTmemSecond = kCols - kShared, kTmemScales = kTmemSecond + kCols;
+    static_assert(kCols % 32 == 0 && kTmemScales + 3 * kTmemScaleSet <= kTmemCols && kShared <= kWarpCols);
     static_assert(kSmemSize <= 232448);
-    static_assert(kChain % 4 == 0 && kMinCut % 4 == 0 && kMinStretch >= 8);
+    static_assert(kChain % 4 == 0 && kWgradMinCut % 4 == 0 && kWgradMinStretch >= 8);
 };
 
 namespace detail {
 
+template <uint32_t kCols>
 __device__ __forceinline__ uint32_t wgrad_tiles_per_group(const WgradParams& p) {
-    return ceil_div(p.n, 128u) * ceil_div(p.k, WgradTile::kBlockFeatures);
+    return ceil_div(p.n, kWgradRows) * ceil_div(p.k, kCols);
 }
 // Length of a tile with so many k-blocks.  Nothing is left to do for an empty group that is added.
 __device__ __forceinline__ uint32_t wgrad_length(const WgradParams& p, uint32_t blocks) {
@@ -220,9 +231,10 @@ __device__ __forceinline__ uint32_t wgrad_length(const WgradParams& p, uint32_t 
 }
 
 // Called by one whole warp.
+template <uint32_t kCols>
 __device__ __forceinline__ void build_wgrad_schedule(const WgradParams& p, WgradSchedule& s) {
     build_token_blocks(p.groups, p.max_blocks, s.blocks);
-    const uint32_t lane = ptx::lane_id(), per_group = wgrad_tiles_per_group(p);
+    const uint32_t lane = ptx::lane_id(), per_group = wgrad_tiles_per_group<kCols>(p);
     uint64_t at = 0;
     for (uint32_t first = 0; first < p.groups.num_groups; first += 32) {
         const uint32_t g = first + lane;
@@ -245,50 +257,52 @@ __device__ __forceinline__ void build_wgrad_schedule(const WgradParams& p, Wgrad
         if (g < p.groups.num_groups)
             s.origin = s.length[g] + static_cast<uint64_t>(p.whole_tiles % per_group) * wgrad_length(p, s.blocks.block[g + 1] - s.blocks.block[g]);
         s.rest = at - s.origin;
-        s.stretches = static_cast<uint32_t>(max(min(static_cast<uint64_t>(gridDim.x), s.rest / WgradTile::kMinStretch), static_cast<uint64_t>(1)));
+        s.stretches = static_cast<uint32_t>(max(min(static_cast<uint64_t>(gridDim.x / 2), s.rest / kWgradMinStretch), static_cast<uint64_t>(1)));
     }
 }
 
-// What one CTA computes at a time: k-blocks [begin, begin + count) of a group, of `blocks`, for one tile of its dW.
+// What a pair computes at a time: k-blocks [begin, begin + count) of a group, of `blocks`, for one tile of its dW.
 struct WgradUnit {
     uint32_t group, row0, col0;        // row0, col0: features of the tile's corner
     uint32_t block0, quad0;            // the group's first k-block and quad of scales
     uint32_t begin, count, blocks;
-    uint32_t first_cta, last_cta;      // who shares the tile
+    uint32_t first_pair, last_pair;    // who shares the tile
 };
 
-// The CTA's units one after the other; every role of the CTA walks them.
+// The pair's units one after the other; every role of both CTAs walks them.
+template <uint32_t kCols>
 struct WgradWalk {
+    uint32_t pair, pairs;
     uint32_t tile;        // next of the dealt tiles
-    uint64_t at, end;     // what is left of the CTA's stretch
+    uint64_t at, end;     // what is left of the pair's stretch
 
-    __device__ __forceinline__ explicit WgradWalk(const WgradSchedule& s)
-        : tile(blockIdx.x),
-          at(blockIdx.x < s.stretches ? s.origin + blockIdx.x * s.rest / s.stretches : 0u),
-          end(blockIdx.x < s.stretches ? s.origin + (blockIdx.x + 1u) * s.rest / s.stretches : 0u) {}
+    __device__ __forceinline__ explicit WgradWalk(const WgradSchedule& s) : pair(blockIdx.x / 2), pairs(gridDim.x / 2), tile(blockIdx.x / 2) {
+        at = pair < s.stretches ? s.origin + pair * s.rest / s.stretches : 0u;
+        end = pair < s.stretches ? s.origin + (pair + 1u) * s.rest / s.stretches : 0u;
+    }
 
     __device__ __forceinline__ static void place(const WgradParams& p, const WgradSchedule& s, uint32_t group, uint32_t in_group, WgradUnit& u) {
-        const uint32_t tiles_n = ceil_div(p.n, 128u), tiles_k = ceil_div(p.k, WgradTile::kBlockFeatures);
-        const uint32_t band = in_group / (16 * tiles_k), in_band = in_group % (16 * tiles_k), rows = min(16u, tiles_n - band * 16);
+        const uint32_t tiles_n = ceil_div(p.n, kWgradRows), tiles_k = ceil_div(p.k, kCols);
+        const uint32_t band = in_group / (8 * tiles_k), in_band = in_group % (8 * tiles_k), rows = min(8u, tiles_n - band * 8);
         u.group = group;
-        u.row0 = (band * 16 + in_band % rows) * 128;
-        u.col0 = in_band / rows * WgradTile::kBlockFeatures;
+        u.row0 = (band * 8 + in_band % rows) * kWgradRows;
+        u.col0 = in_band / rows * kCols;
         u.block0 = s.blocks.block[group];
         u.quad0 = s.blocks.quad[group];
         u.blocks = s.blocks.block[group + 1] - u.block0;
     }
-    // The CTA in whose stretch a position lies.
+    // The pair in whose stretch a position lies.
     __device__ __forceinline__ static uint32_t owner(const WgradSchedule& s, uint64_t position) {
         return static_cast<uint32_t>(((position - s.origin + 1) * s.stretches - 1) / s.rest);
     }
 
     __device__ __forceinline__ bool next(const WgradParams& p, const WgradSchedule& s, WgradUnit& u) {
-        const uint32_t per_group = wgrad_tiles_per_group(p);
+        const uint32_t per_group = wgrad_tiles_per_group<kCols>(p);
         if (tile < p.whole_tiles) {
             place(p, s, tile / per_group, tile % per_group, u);
             u.begin = 0, u.count = u.blocks;
-            u.first_cta = u.last_cta = blockIdx.x;
-            tile += gridDim.x;
+            u.first_pair = u.last_pair = pair;
+            tile += pairs;
             return true;
         }
         while (at < end) {
@@ -305,17 +319,17 @@ struct WgradWalk {
             const uint64_t until = end - start;
             at = start + length;
             place(p, s, low, in_group, u);
-            if (blocks < WgradTile::kMinCut) {
+            if (blocks < kWgradMinCut) {
                 if (from != 0) continue;
                 u.begin = 0, u.count = blocks;
-                u.first_cta = u.last_cta = blockIdx.x;
+                u.first_pair = u.last_pair = pair;
                 return true;
             }
             u.begin = from >= blocks ? blocks : from & ~3u;
             u.count = (until >= blocks ? blocks : static_cast<uint32_t>(until) & ~3u) - u.begin;
             if (u.count == 0) continue;
-            u.first_cta = owner(s, start + 3);  // a stretch that ends in the first three k-blocks has none of them
-            u.last_cta = owner(s, start + blocks - 1);
+            u.first_pair = owner(s, start + 3);  // a stretch that ends in the first three k-blocks has none of them
+            u.last_pair = owner(s, start + blocks - 1);
             return true;
         }
         return false;
@@ -334,19 +348,22 @@ __device__ __forceinline__ void red_add4(float* p, const uint4& v) {
                  : "memory");
 }
 
-// Stores a warp's 32 rows x 128 columns; lane r holds row r.  The rows go through the warp's box in shared memory, 16 columns at a time in
+// Stores a warp's 32 rows x kWarpCols columns; lane r holds row r, acc[c] column first_col + c / 16 * 16 * direction + c % 16.  The rows go through the warp's box in shared memory, 16 columns at a time in
 // fp32, so that a store instruction covers eight pieces of 64 contiguous bytes.  fp32 is added to what dW holds where dW lies, in L2:
-// every element once, so that the order does not matter, and nothing waits for the old value (16 experts N=4096 K=2048, 16384 tokens:
-// 535 us with loads and stores).  bf16 is loaded, added in 32 bits and rounded once.
-template <typename out_t>
-__device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const WgradUnit& u, uint32_t box, uint32_t row_in_tile, uint32_t col0,
-                                                 uint32_t lane, const float (&acc)[128]) {
+// every element once, so that the order does not matter, and nothing waits for the old value.  That is what bounds an accumulated tile
+// with few tokens: L2 adds 2.2 TB/s (16 experts N=4096 K=2048, 16384 tokens: 240 us; loads and stores at the end of a tile 535, loads of
+// the next tile's old values ahead of its products, from L2 as a prefetch left them, 372).  bf16 is loaded, added in 32 bits and
+// rounded once.
+template <typename out_t, uint32_t kWarpCols>
+__device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const WgradUnit& u, uint32_t box, uint32_t row_in_tile, uint32_t first_col,
+                                                 uint32_t direction, uint32_t lane, const float (&acc)[kWarpCols]) {
     out_t* out = reinterpret_cast<out_t*>(p.out) + u.group * p.out_group;
     const uint32_t row0 = u.row0 + row_in_tile;
-    if (u.col0 + col0 >= p.k || row0 >= p.n) return;
+    if (row0 >= p.n) return;
 #pragma unroll
-    for (uint32_t pass = 0; pass < 8; ++pass) {
-        const uint32_t chunk = lane % 4, col = u.col0 + col0 + pass * 16 + chunk * 4;
+    for (uint32_t pass = 0; pass < kWarpCols / 16; ++pass) {
+        const uint32_t col0 = u.col0 + first_col + pass * 16 * direction, chunk = lane % 4, col = col0 + chunk * 4;
+        if (col0 >= p.k) continue;
         [[maybe_unused]] uint2 old[4];
         if constexpr (sizeof(out_t) == 2) {
             if (p.vector_store != 0 && p.accumulate != 0) {
@@ -389,7 +406,7 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
             }
         } else {
             // one element per lane, two rows at a time
-            const uint32_t c = lane % 16, column = u.col0 + col0 + pass * 16 + c;
+            const uint32_t c = lane % 16, column = col0 + c;
 #pragma unroll 4
             for (uint32_t r = lane / 16; r < 32; r += 2) {
                 const float v = ptx::ld_shared_f32(box + r * 64 + (((c / 4) ^ ((r >> 1) & 3u)) << 4) + c % 4 * 4);
@@ -408,25 +425,33 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
 
 }  // namespace detail
 
-template <typename out_t>
-__global__ void __launch_bounds__(384, 1)
-    fp8_wgrad_kernel(const WgradParams p, const __grid_constant__ CUtensorMap map_n, const __grid_constant__ CUtensorMap map_k) {
+struct WgradMaps {
+    CUtensorMap n, k;                // codes of dy and x: boxes of 128 tokens x 128 features
+    CUtensorMap scales_n, scales_k;  // their scale tiles: a box is what a tile of products needs
+};
+
+template <uint32_t kCols, typename out_t>
+__global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
+    fp8_wgrad_kernel(const WgradParams p, const __grid_constant__ WgradMaps maps) {
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
-    using T = WgradTile;
+    using T = WgradTile<kCols>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
     WgradSchedule& schedule = *reinterpret_cast<WgradSchedule*>(smem + T::kOffSchedule);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + T::kOffBarriers);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + T::kOffBarriers);  // of rank 0 alone, for the loads of both
     uint64_t* empty = full + T::kStages;
     uint64_t* sums_full = empty + T::kStages;
-    uint64_t* sums_empty = sums_full + 1;
+    uint64_t* sums_empty = sums_full + 2;    // of rank 0 alone: all columns have been read
+    uint64_t* shared_empty = sums_empty + 2;  // of rank 0 alone: those that both accumulators use
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + T::kOffTmemSlot);
     volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + T::kOffAbort);
-    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = ptx::lane_id();
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = ptx::lane_id(), rank = ptx::cluster_ctarank();
 
     if (warp == 0 && lane == 0 && p.max_blocks != 0) {
-        ptx::tma_prefetch_desc(&map_n);
-        ptx::tma_prefetch_desc(&map_k);
+        ptx::tma_prefetch_desc(&maps.n);
+        ptx::tma_prefetch_desc(&maps.k);
+        ptx::tma_prefetch_desc(&maps.scales_n);
+        ptx::tma_prefetch_desc(&maps.scales_k);
     }
     if (warp == 1 && lane == 0) {
 #pragma unroll
@@ -434,35 +459,41 @@ __global__ void __launch_bounds__(384, 1)
             ptx::mbar_init(full + i, 1);
             ptx::mbar_init(empty + i, 1);
         }
-        ptx::mbar_init(sums_full, 1);
-        ptx::mbar_init(sums_empty, 8);  // one arrival per warp that reads the sums
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            ptx::mbar_init(sums_full + i, 1);
+            ptx::mbar_init(sums_empty + i, 16);  // one arrival per warp that reads the sums, in both CTAs
+            ptx::mbar_init(shared_empty + i, 8);  // half of them read the shared columns
+        }
         *abort_flag = 0;
         ptx::fence_barrier_init();
         ptx::fence_proxy_async_smem();
     }
     ptx::grid_dependency_wait();
-    if (warp == 3) detail::build_wgrad_schedule(p, schedule);
+    if (warp == 3) detail::build_wgrad_schedule<kCols>(p, schedule);
     if (warp == 2) {
-        ptx::tmem_alloc(tmem_slot, T::kTmemCols);
-        ptx::tmem_relinquish_alloc_permit();
+        ptx::tmem_alloc_pair(tmem_slot, T::kTmemCols);
+        ptx::tmem_relinquish_alloc_permit_pair();
     }
     ptx::tcgen05_fence_before_thread_sync();
     __syncthreads();
+    ptx::cluster_arrive(), ptx::cluster_wait();  // the other CTA's barriers and tensor memory are ready
     ptx::tcgen05_fence_after_thread_sync();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t tiles_n = ceil_div(p.n, 128u), tiles_k128 = ceil_div(p.k, 128u);
-    detail::WgradWalk walk(schedule);
+    detail::WgradWalk<kCols> walk(schedule);
     detail::WgradUnit u;
 
     if (warp < 4) {
         ptx::reg_dealloc<56>();
-        if (warp == 0 && lane == 0) {
-            // ---- loads: a k-block of both operands per stage, and the scales of four k-blocks with the first of them ----
+        if (warp == 0 && ptx::elect_one()) {
+            // ---- loads: each CTA its rows of A and its half of B's columns per k-block, and with the first of four k-blocks its rows'
+            // scales and all columns' ----
+            const uint32_t tiles_n = ceil_div(p.n, 128u), tiles_k = ceil_div(p.k, kCols);
+            const uint32_t full_of_pair = ptx::map_to_cta(ptx::smem_u32(full), 0);
             uint32_t stage = 0, phase = 0;
             bool alive = true;
             while (alive && walk.next(p, schedule, u)) {
-                const bool second_box = u.col0 + 128 < p.k;
-                const uint32_t boxes = second_box ? 2 : 1;
+                const uint32_t row = u.row0 + rank * 128, col = u.col0 + rank * (kCols / 2);
                 for (uint32_t i = 0; i < u.count; ++i) {
                     const uint32_t kb = u.begin + i;
                     if (!detail::bounded_wait(empty + stage, phase ^ 1, abort_flag, p, 17)) {
@@ -470,18 +501,19 @@ __global__ void __launch_bounds__(384, 1)
                         break;
                     }
                     const bool scales = i == 0 || kb % 4 == 0;
-                    ptx::mbar_arrive_expect_tx(full + stage, kMnBoxBytes * (1 + boxes) + (scales ? kScaleTileBytes * (1 + boxes) : 0u));
+                    if (rank == 0)
+                        ptx::mbar_arrive_expect_tx(full + stage, 2 * (T::kStageA + T::kStageB + (scales ? T::kStageScales : 0u)));
                     const int32_t token = static_cast<int32_t>((u.block0 + kb) * 128);
-                    uint8_t* b = smem + T::kOffB + stage * T::kStageB;
-                    ptx::tma_load_2d(smem + T::kOffA + stage * T::kStageA, &map_n, full + stage, static_cast<int32_t>(u.row0), token);
-                    ptx::tma_load_2d(b, &map_k, full + stage, static_cast<int32_t>(u.col0), token);
-                    if (second_box) ptx::tma_load_2d(b + kMnBoxBytes, &map_k, full + stage, static_cast<int32_t>(u.col0 + 128), token);
+                    const uint32_t bar = full_of_pair + stage * 8;
+                    ptx::tma_load_2d_pair(smem + T::kOffA + stage * T::kStageA, &maps.n, bar, static_cast<int32_t>(row), token);
+                    ptx::tma_load_2d_pair(smem + T::kOffB + stage * T::kStageB, &maps.k, bar, static_cast<int32_t>(col), token);
                     if (scales) {
-                        const uint64_t quad = u.quad0 + kb / 4;
+                        const uint32_t quad = u.quad0 + kb / 4;
                         uint8_t* s = smem + T::kOffScales + stage * T::kStageScales;
-                        ptx::bulk_load(s, p.scales_n + (quad * tiles_n + u.row0 / 128) * kScaleTileBytes, kScaleTileBytes, full + stage);
-                        ptx::bulk_load(s + kScaleTileBytes, p.scales_k + (quad * tiles_k128 + u.col0 / 128) * kScaleTileBytes,
-                                       kScaleTileBytes * boxes, full + stage);
+                        // rows that dW does not have: any scales will do
+                        ptx::tma_load_2d_pair(s, &maps.scales_n, bar, 0, static_cast<int32_t>(quad * tiles_n + min(row / 128, tiles_n - 1)));
+                        ptx::tma_load_2d_pair(s + kScaleTileBytes, &maps.scales_k, bar, 0,
+                                              static_cast<int32_t>((quad * tiles_k + u.col0 / kCols) * (T::kScaleTiles - 1)));
                     }
                     if (++stage == T::kStages) {
                         stage = 0;
@@ -490,110 +522,132 @@ __global__ void __launch_bounds__(384, 1)
                 }
             }
             if (!alive) detail::drain_copies();
-        } else if (warp == 1 && lane == 0) {
-            // ---- products ----
-            constexpr uint32_t idesc = make_instr_desc_mx_mn_major(128, T::kBlockFeatures);
-            uint32_t stage = 0, phase = 0, sums_phase = 0, set = 0;
-            bool alive = true;
+        } else if (warp == 1 && rank == 0 && ptx::elect_one()) {
+            // ---- products of the pair ----
+            constexpr uint32_t idesc = make_instr_desc_mx_mn_major(kWgradRows, kCols);
+            const uint32_t a_low = make_smem_desc_mn_major_low(ptx::smem_u32(smem + T::kOffA));
+            const uint32_t b_low = make_smem_desc_mn_major_low(ptx::smem_u32(smem + T::kOffB));
+            const uint64_t scales_desc = make_smem_desc_scales(ptx::smem_u32(smem + T::kOffScales));
+            uint32_t stage = 0, phase = 0, buf = 0, sums_phase = 0, set = 0;
+            bool alive = true, loaded = false;  // loaded: the next stage was seen to be full already
             while (alive && walk.next(p, schedule, u)) {
+                uint32_t left_in_chain = 0;
                 for (uint32_t i = 0; i < u.count; ++i) {
                     const uint32_t kb = u.begin + i;
-                    if (i % T::kChain == 0) {
-                        if (!detail::bounded_wait(sums_empty, sums_phase ^ 1, abort_flag, p, 18)) {
+                    const bool begins = left_in_chain == 0;
+                    if (begins) {
+                        left_in_chain = min(T::kChain, u.count - i);
+                        // this accumulator's sums of two chains ago, and the other's in the columns that both use
+                        if (!detail::bounded_wait(sums_empty + buf, sums_phase ^ 1, abort_flag, p, 18) ||
+                            (T::kShared != 0 && !detail::bounded_wait(shared_empty + (buf ^ 1), buf == 0 ? sums_phase ^ 1 : sums_phase, abort_flag, p, 21))) {
                             alive = false;
                             break;
                         }
-                        sums_phase ^= 1;
                     }
-                    if (!detail::bounded_wait(full + stage, phase, abort_flag, p, 19)) {
+                    if (!loaded && !detail::bounded_wait(full + stage, phase, abort_flag, p, 19)) {
                         alive = false;
                         break;
                     }
                     ptx::tcgen05_fence_after_thread_sync();
-                    if (i == 0 || kb % 4 == 0) {
-                        // Two sets in turn: the set that is written now was last used two quads ago, and a stage is loaded again only when
-                        // its products are complete, four k-blocks ago; a tile begins when the one in front is complete.
-                        set ^= 1;
-                        const uint32_t s = ptx::smem_u32(smem + T::kOffScales + stage * T::kStageScales);
-#pragma unroll
-                        for (uint32_t t = 0; t < T::kScaleTiles; ++t)
-                            ptx::tmem_copy_scales(tmem + T::kTmemScales + set * T::kTmemScaleSet + t * 4,
-                                                  make_smem_desc_scales(s + t * kScaleTileBytes));
-                    }
-                    const uint64_t a = make_smem_desc_mn_major_sw128(ptx::smem_u32(smem + T::kOffA + stage * T::kStageA));
-                    const uint64_t b = make_smem_desc_mn_major_sw128(ptx::smem_u32(smem + T::kOffB + stage * T::kStageB));
-                    const uint32_t scale_a = tmem + T::kTmemScales + set * T::kTmemScaleSet;
-#pragma unroll
-                    for (uint32_t s = 0; s < 4; ++s)
-                        ptx::umma_mxf8f6f4_ss(tmem, a + s * kMnKStep, b + s * kMnKStep, with_scale_byte(idesc, kb % 4), scale_a, scale_a + 4,
-                                              i % T::kChain != 0 || s != 0);
-                    ptx::umma_commit(empty + stage);
-                    if (i % T::kChain == T::kChain - 1 || i + 1 == u.count) ptx::umma_commit(sums_full);
+                    const uint32_t now = stage;
                     if (++stage == T::kStages) {
                         stage = 0;
                         phase ^= 1;
+                    }
+                    loaded = ptx::mbar_test_wait(full + stage, phase);
+                    if (i == 0 || kb % 4 == 0) {
+                        // Three sets in turn.  The set that is written now was last used three quads ago.  If that was in this chain or the
+                        // one in front, at least five k-blocks lie in between, and the stage just filled was free: the products of six
+                        // k-blocks ago are complete.  If it was earlier, its accumulator has been read.
+                        set = set == 2 ? 0 : set + 1;
+#pragma unroll
+                        for (uint32_t t = 0; t < T::kScaleTiles; ++t)
+                            ptx::tmem_copy_scales_pair(tmem + T::kTmemScales + set * T::kTmemScaleSet + t * 4,
+                                                       scales_desc + ((now * T::kStageScales + t * kScaleTileBytes) >> 4));
+                    }
+                    const uint32_t a = a_low + now * (T::kStageA >> 4), b = b_low + now * (T::kStageB >> 4);
+                    const uint32_t scale_a = tmem + T::kTmemScales + set * T::kTmemScaleSet, sums = tmem + buf * T::kTmemSecond;
+                    const uint32_t desc = with_scale_byte(idesc, kb % 4);
+#pragma unroll
+                    for (uint32_t s = 0; s < 4; ++s)
+                        ptx::umma_mxf8f6f4_ss_pair(sums, a + s * kMnKStep, b + s * kMnKStep, desc, scale_a, scale_a + 4, !begins || s != 0);
+                    ptx::umma_commit_pair(empty + now);
+                    if (--left_in_chain == 0) {
+                        ptx::umma_commit_pair(sums_full + buf);
+                        buf ^= 1;
+                        if (buf == 0) sums_phase ^= 1;
                     }
                 }
             }
         }
         __syncwarp();
     } else {
-        // ---- sums -> dW ----
+        // ---- sums -> dW: this CTA's 128 rows ----
         ptx::reg_alloc<224>();  // 128 * 56 + 256 * 224 = 384 * 168, the launch's registers
-        const uint32_t quarter = warp % 4, part = warp - 4, col0 = part / 4 * 128;
+        constexpr uint32_t kWarpCols = T::kWarpCols;
+        const uint32_t quarter = warp % 4, part = warp - 4;
+        // 16 columns at a time, the warps of the first half upwards and those of the second downwards: each begins with the columns that
+        // both accumulators use.  acc[c] belongs to column first_col + c / 16 * 16 * direction + c % 16.
+        const uint32_t first_col = part < 4 ? 0 : kCols - 16, direction = part < 4 ? 1 : ~0u;
         const uint32_t box = ptx::smem_u32(smem + T::kOffStore + part * T::kBoxBytes);
-        uint32_t sums_phase = 0;
+        const uint32_t empty_of_pair = ptx::map_to_cta(ptx::smem_u32(sums_empty), 0);
+        [[maybe_unused]] const uint32_t shared_of_pair = ptx::map_to_cta(ptx::smem_u32(shared_empty), 0);
+        uint32_t buf = 0, sums_phase = 0;
         bool alive = true;
         while (alive && walk.next(p, schedule, u)) {
-            float acc[128];
+            float acc[kWarpCols];
 #pragma unroll
-            for (uint32_t j = 0; j < 128; ++j) acc[j] = 0.0f;
+            for (uint32_t j = 0; j < kWarpCols; ++j) acc[j] = 0.0f;
 #pragma unroll 1
             for (uint32_t i = 0; i < u.count; i += T::kChain) {
-                const bool ok = detail::bounded_wait(sums_full, sums_phase, abort_flag, p, 20);
+                const bool ok = detail::bounded_wait(sums_full + buf, sums_phase, abort_flag, p, 20);
                 if (!__all_sync(0xffffffffu, ok)) {
                     alive = false;
                     break;
                 }
-                sums_phase ^= 1;
                 ptx::tcgen05_fence_after_thread_sync();
+                const uint32_t from = tmem + ((quarter * 32u) << 16) + buf * T::kTmemSecond + first_col;
 #pragma unroll
-                for (uint32_t c = 0; c < 128; c += 32) {
-                    uint32_t t[32];
-                    ptx::tmem_ld_32x32b<32>(tmem + ((quarter * 32u) << 16) + col0 + c, t);
-                    ptx::tmem_ld_wait<32>(t);
-                    if (c == 96) {
+                for (uint32_t c = 0; c < kWarpCols; c += 16) {
+                    uint32_t t[16];
+                    ptx::tmem_ld_32x32b<16>(from + c * direction, t);
+                    ptx::tmem_ld_wait<16>(t);
+                    const bool last = c + 16 == kWarpCols;
+                    if (last || (T::kShared != 0 && c + 16 == T::kShared)) {
                         ptx::tcgen05_fence_before_thread_sync();
                         __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive(sums_empty);
+                        if (lane == 0 && (last || (buf == 0) == (part >= 4))) ptx::mbar_arrive_cluster((last ? empty_of_pair : shared_of_pair) + buf * 8);
                     }
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; ++j) acc[c + j] += __uint_as_float(t[j]);
+                    for (uint32_t j = 0; j < 16; ++j) acc[c + j] += __uint_as_float(t[j]);
                 }
+                buf ^= 1;
+                if (buf == 0) sums_phase ^= 1;
             }
             if (!alive || *abort_flag != 0) break;  // a wait ran out: the sums may be incomplete
-            if (u.first_cta != u.last_cta) {
-                // Partial tiles meet in L2; who counts itself last adds them in the order of the tokens.  A CTA begins at most one tile
+            if (u.first_pair != u.last_pair) {
+                // Partial tiles meet in L2; who counts itself last adds them in the order of the tokens.  A pair begins at most one tile
                 // that others end, and ends at most one that another began: a slot for each.
-                auto slot = [&](uint32_t cta) {
-                    return p.partials + (static_cast<uint64_t>(2 * cta + (cta == u.first_cta ? 1 : 0)) * 8 + part) * 1024 + lane;
+                auto slot = [&](uint32_t pair) {
+                    return p.partials + ((static_cast<uint64_t>(2 * pair + (pair == u.first_pair ? 1 : 0)) * 2 + rank) * 8 + part) * (kWarpCols / 4 * 32) + lane;
                 };
-                float4* mine = slot(blockIdx.x);
+                float4* mine = slot(walk.pair);
 #pragma unroll
-                for (uint32_t j = 0; j < 32; ++j) __stcg(mine + j * 32, make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]));
+                for (uint32_t j = 0; j < kWarpCols / 4; ++j)
+                    __stcg(mine + j * 32, make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]));
                 __threadfence();
                 __syncwarp();
                 uint32_t before = 0;
-                if (lane == 0) before = atomicAdd(p.counters + u.first_cta * 8 + part, 1u);
-                if (__shfl_sync(0xffffffffu, before, 0) != u.last_cta - u.first_cta) continue;
+                if (lane == 0) before = atomicAdd(p.counters + (u.first_pair * 2 + rank) * 8 + part, 1u);
+                if (__shfl_sync(0xffffffffu, before, 0) != u.last_pair - u.first_pair) continue;
                 __threadfence();
 #pragma unroll
-                for (uint32_t j = 0; j < 128; ++j) acc[j] = 0.0f;
+                for (uint32_t j = 0; j < kWarpCols; ++j) acc[j] = 0.0f;
 #pragma unroll 1
-                for (uint32_t cta = u.first_cta; cta <= u.last_cta; ++cta) {
-                    const float4* from = slot(cta);
+                for (uint32_t pair = u.first_pair; pair <= u.last_pair; ++pair) {
+                    const float4* from = slot(pair);
 #pragma unroll
-                    for (uint32_t j = 0; j < 32; ++j) {
+                    for (uint32_t j = 0; j < kWarpCols / 4; ++j) {
                         const float4 f = __ldcg(from + j * 32);
                         acc[4 * j] += f.x, acc[4 * j + 1] += f.y, acc[4 * j + 2] += f.z, acc[4 * j + 3] += f.w;
                     }
@@ -601,15 +655,16 @@ __global__ void __launch_bounds__(384, 1)
             } else if (u.blocks == 0 && p.accumulate != 0) {
                 continue;
             }
-            detail::store_wgrad_rows<out_t>(p, u, box, quarter * 32, col0, lane, acc);
+            detail::store_wgrad_rows<out_t, kWarpCols>(p, u, box, rank * 128 + quarter * 32, first_col, direction, lane, acc);
         }
         __syncwarp();
     }
     ptx::tcgen05_fence_before_thread_sync();
     __syncthreads();
+    ptx::cluster_arrive(), ptx::cluster_wait();  // neither CTA's memory is needed by the other any more
     if (warp == 2) {
         ptx::tcgen05_fence_after_thread_sync();
-        ptx::tmem_dealloc(tmem, T::kTmemCols);
+        ptx::tmem_dealloc_pair(tmem, T::kTmemCols);
     }
 #endif
 }
@@ -636,30 +691,38 @@ struct WgradArgs {
 // What lies in the workspace, in this order, each on a 256-byte boundary.
 struct WgradWorkspace {
     size_t codes_n, codes_k, scales_n, scales_k, counters, partials, bytes;
-    uint32_t codes_ld_n, codes_ld_k, blocks, tiles, whole_tiles, ctas, num_counters;
+    uint32_t codes_ld_n, codes_ld_k, blocks, quads, cols, tiles, whole_tiles, pairs, num_counters;
 };
 
 // How many tiles are dealt out whole (see WgradSchedule): full waves, one less where more than half of another wave is left, because that
 // one would run nearly as long as a full one.
-inline uint32_t choose_whole_wgrad_tiles(uint32_t tiles, uint32_t ctas) {
-    const uint32_t waves = tiles / ctas, rest = tiles % ctas;
-    return (2 * rest > ctas && waves > 0 ? waves - 1 : waves) * ctas;
+inline uint32_t choose_whole_wgrad_tiles(uint32_t tiles, uint32_t pairs) {
+    const uint32_t waves = tiles / pairs, rest = tiles % pairs;
+    return (2 * rest > pairs && waves > 0 ? waves - 1 : waves) * pairs;
+}
+
+// Columns of a tile: 256 unless tiles of 192 overhang dW less.
+inline uint32_t choose_wgrad_cols(uint32_t k) {
+    return align_up(k, 192u) * 1.05 < align_up(k, 256u) ? 192 : 256;
 }
 
 inline bool plan_wgrad_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t groups, bool grouped, uint32_t num_sms, WgradWorkspace& w) {
     w.blocks = max_token_blocks(rows, groups, grouped);
     w.codes_ld_n = align_up(n, 16u);
     w.codes_ld_k = align_up(k, 16u);
-    const uint64_t tiles = static_cast<uint64_t>(ceil_div(n, 128u)) * ceil_div(k, WgradTile::kBlockFeatures) * groups;
+    w.cols = choose_wgrad_cols(k);
+    const uint64_t tiles = static_cast<uint64_t>(ceil_div(n, kWgradRows)) * ceil_div(k, w.cols) * groups;
     if (tiles > 0x7fffffffull || static_cast<uint64_t>(w.blocks) * 128 > 0x7fffffffull || num_sms == 0) return false;
     w.tiles = static_cast<uint32_t>(tiles);
-    // a CTA per tile, or per kMinCut k-blocks of one
-    const uint64_t useful = tiles * (1 + w.blocks / WgradTile::kMinCut);
-    w.ctas = useful < num_sms ? static_cast<uint32_t>(useful) : num_sms;
-    w.whole_tiles = choose_whole_wgrad_tiles(w.tiles, w.ctas);
-    const bool shared = w.whole_tiles != w.tiles && w.blocks >= WgradTile::kMinCut;  // tiles may be cut
-    const uint64_t quads = max_token_quads(w.blocks, groups);
-    w.num_counters = shared ? w.ctas * 8 : 0;
+    // a pair per tile, or per kWgradMinCut k-blocks of one
+    const uint64_t useful = tiles * (1 + w.blocks / kWgradMinCut), pairs = num_sms > 1 ? num_sms / 2 : 1;
+    w.pairs = static_cast<uint32_t>(useful < pairs ? useful : pairs);
+    w.whole_tiles = choose_whole_wgrad_tiles(w.tiles, w.pairs);
+    const bool shared = w.whole_tiles != w.tiles && w.blocks >= kWgradMinCut;  // tiles may be cut
+    const uint64_t quads = max_token_quads(w.blocks, groups), scale_rows = quads * (ceil_div(n, 128u) + 2ull * ceil_div(k, w.cols));
+    if (scale_rows > 0x7fffffffull) return false;
+    w.quads = static_cast<uint32_t>(quads);
+    w.num_counters = shared ? w.pairs * 16 : 0;
     size_t at = 0;
     auto take = [&at](size_t bytes) {
         const size_t here = at;
@@ -669,11 +732,50 @@ inline bool plan_wgrad_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t
     w.codes_n = take(static_cast<size_t>(w.blocks) * 128 * w.codes_ld_n);
     w.codes_k = take(static_cast<size_t>(w.blocks) * 128 * w.codes_ld_k);
     w.scales_n = take(quads * ceil_div(n, 128u) * kScaleTileBytes);
-    w.scales_k = take(quads * ceil_div(k, 128u) * kScaleTileBytes);
+    w.scales_k = take(quads * ceil_div(k, w.cols) * 2 * kScaleTileBytes);
     w.counters = take(w.num_counters * sizeof(uint32_t));
-    w.partials = take(shared ? static_cast<size_t>(2) * w.ctas * 128 * WgradTile::kBlockFeatures * sizeof(float) : 0);
+    w.partials = take(shared ? static_cast<size_t>(2) * w.pairs * kWgradRows * w.cols * sizeof(float) : 0);
     w.bytes = at;
     return true;
+}
+
+// Scale tiles as rows of 128 words; a box is `rows` of them.
+inline CUtensorMap make_scale_tiles_desc(const void* base, uint64_t tiles, uint32_t rows, bool& ok) {
+    CUtensorMap map{};
+    EncodeTiledFn encode = get_encode_tiled();
+    const cuuint64_t dims[2] = {kScaleTileBytes / 4, tiles}, strides[1] = {kScaleTileBytes};
+    const cuuint32_t box[2] = {kScaleTileBytes / 4, rows}, elem_strides[2] = {1, 1};
+    if (encode == nullptr || encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, elem_strides,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        ok = false;
+    return map;
+}
+
+template <uint32_t kCols, typename out_t>
+inline int launch_wgrad_products(const WgradParams& p, const WgradMaps& maps, uint32_t pairs, cudaStream_t stream) {
+    constexpr uint32_t kSmem = WgradTile<kCols>::kSmemSize;
+    int device = 0, max_smem = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return kLaunchFailed;
+    cudaDeviceGetAttribute(&max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+    if (static_cast<int>(kSmem) > max_smem) return kSmemTooLarge;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * pairs);
+    cfg.blockDim = dim3(384);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    auto kernel = fp8_wgrad_kernel<kCols, out_t>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)) != cudaSuccess ||
+        cudaLaunchKernelEx(&cfg, kernel, p, maps) != cudaSuccess) {
+        cudaGetLastError();
+        return kLaunchFailed;
+    }
+    return kOk;
 }
 
 inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
@@ -687,82 +789,71 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
     if (!plan_wgrad_workspace(a.groups.rows, a.n, a.k, a.groups.num_groups, grouped, static_cast<uint32_t>(a.num_sms), w)) return kBadArgument;
     if (w.bytes != 0 && (a.workspace == nullptr || !is_aligned(a.workspace, 256))) return kBadArgument;
     if (a.workspace_bytes < w.bytes) return kWorkspaceTooSmall;
-    int device = 0, sm_count = 0, max_smem = 0;
+    if (w.blocks > 65535) return kBadArgument;  // the cast's grid
+    int device = 0, sm_count = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return kLaunchFailed;
     cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device);
-    cudaDeviceGetAttribute(&max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
     if (a.num_sms > sm_count) return kBadArgument;
-    if (static_cast<int>(WgradTile::kSmemSize) > max_smem) return kSmemTooLarge;
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
 
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-
-    const uint32_t tiles_n = ceil_div(a.n, 128u), tiles_k128 = ceil_div(a.k, 128u);
+    WgradMaps maps = {};
     if (w.blocks != 0) {
+        bool ok = true;
+        maps.n = make_2d_tma_desc_u8_sw128(ws + w.codes_n, static_cast<uint64_t>(w.blocks) * 128, a.n, w.codes_ld_n, 128, ok);
+        maps.k = make_2d_tma_desc_u8_sw128(ws + w.codes_k, static_cast<uint64_t>(w.blocks) * 128, a.k, w.codes_ld_k, 128, ok);
+        maps.scales_n = make_scale_tiles_desc(ws + w.scales_n, static_cast<uint64_t>(w.quads) * ceil_div(a.n, 128u), 1, ok);
+        maps.scales_k = make_scale_tiles_desc(ws + w.scales_k, static_cast<uint64_t>(w.quads) * ceil_div(a.k, w.cols) * 2, 2, ok);
+        if (!ok) return kTensorMapFailed;
+
         CastTokensParams c;
         c.groups = a.groups;
         c.max_blocks = w.blocks;
-        auto operand = [](const void* z, uint64_t ld, uint32_t cols, uint8_t* codes, uint32_t codes_ld, uint8_t* scales) {
+        auto operand = [](const void* z, uint64_t ld, uint32_t cols, uint8_t* codes, uint32_t codes_ld, uint8_t* scales, uint32_t scale_cols) {
             CastTokensOperand o;
             o.z = static_cast<const __nv_bfloat16*>(z);
             o.ld = ld, o.cols = cols;
             o.wide = is_aligned(z, 32) && ld % 16 == 0 && cols % 16 == 0;
-            o.codes = codes, o.codes_ld = codes_ld, o.scales = scales;
+            o.codes = codes, o.codes_ld = codes_ld, o.scales = scales, o.scale_cols = scale_cols;
             return o;
         };
-        c.operand[0] = operand(a.dy, a.dy_ld, a.n, ws + w.codes_n, w.codes_ld_n, ws + w.scales_n);
-        c.operand[1] = operand(a.x, a.x_ld, a.k, ws + w.codes_k, w.codes_ld_k, ws + w.scales_k);
-        c.column_tiles[0] = tiles_n, c.column_tiles[1] = tiles_k128;
+        c.operand[0] = operand(a.dy, a.dy_ld, a.n, ws + w.codes_n, w.codes_ld_n, ws + w.scales_n, 128);
+        c.operand[1] = operand(a.x, a.x_ld, a.k, ws + w.codes_k, w.codes_ld_k, ws + w.scales_k, w.cols);
+        c.column_tiles[0] = ceil_div(a.n, 128u), c.column_tiles[1] = ceil_div(a.k, 128u);
         c.counters = reinterpret_cast<uint32_t*>(ws + w.counters);
         c.num_counters = w.num_counters;
-        if (w.blocks > 65535) return kBadArgument;
-        cfg.gridDim = dim3(tiles_n + tiles_k128, w.blocks);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(c.column_tiles[0] + c.column_tiles[1], w.blocks);
         cfg.blockDim = dim3(256);
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
         if (cudaLaunchKernelEx(&cfg, block_cast_tokens_kernel, c) != cudaSuccess) {
             cudaGetLastError();
             return kLaunchFailed;
         }
     }
 
-    bool ok = true;
-    CUtensorMap map_n{}, map_k{};
-    if (w.blocks != 0) {
-        map_n = make_2d_tma_desc_u8_sw128(ws + w.codes_n, static_cast<uint64_t>(w.blocks) * 128, a.n, w.codes_ld_n, 128, ok);
-        map_k = make_2d_tma_desc_u8_sw128(ws + w.codes_k, static_cast<uint64_t>(w.blocks) * 128, a.k, w.codes_ld_k, 128, ok);
-    }
-    if (!ok) return kTensorMapFailed;
     WgradParams p;
     p.groups = a.groups;
     p.max_blocks = w.blocks;
     p.n = a.n, p.k = a.k;
-    p.scales_n = ws + w.scales_n, p.scales_k = ws + w.scales_k;
     p.out = a.out, p.out_ld = a.out_ld, p.out_group = a.out_group;
     p.accumulate = a.accumulate;
     const uint32_t vec = 4, item = a.out_bf16 ? 2 : 4;  // four columns at a time
     p.vector_store = is_aligned(a.out, vec * item) && a.out_ld % vec == 0 && a.out_group % vec == 0 && a.k % vec == 0;
     p.tiles = w.tiles, p.whole_tiles = w.whole_tiles;
-    // A tile of 128 KB in fp32 leaves at 1/148 of the memory's rate in the time of about ten k-blocks.
+    // A CTA's 128 rows of a tile, about 100 KB in fp32, leave at 1/148 of the memory's rate in the time of about ten k-blocks.
     p.store_cost = (a.out_bf16 ? 5u : 10u) * (a.accumulate ? 2u : 1u);
     p.partials = reinterpret_cast<float4*>(ws + w.partials);
     p.counters = reinterpret_cast<uint32_t*>(ws + w.counters);
     p.status = a.status;
     p.timeout_ns = a.timeout_ns;
-    cfg.gridDim = dim3(w.ctas);
-    cfg.blockDim = dim3(384);
-    cfg.dynamicSmemBytes = WgradTile::kSmemSize;
-    auto kernel = a.out_bf16 ? fp8_wgrad_kernel<__nv_bfloat16> : fp8_wgrad_kernel<float>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(WgradTile::kSmemSize)) != cudaSuccess ||
-        cudaLaunchKernelEx(&cfg, kernel, p, map_n, map_k) != cudaSuccess) {
-        cudaGetLastError();
-        return kLaunchFailed;
-    }
-    return kOk;
+    if (w.cols == 192)
+        return a.out_bf16 ? launch_wgrad_products<192, __nv_bfloat16>(p, maps, w.pairs, stream) : launch_wgrad_products<192, float>(p, maps, w.pairs, stream);
+    return a.out_bf16 ? launch_wgrad_products<256, __nv_bfloat16>(p, maps, w.pairs, stream) : launch_wgrad_products<256, float>(p, maps, w.pairs, stream);
 }
 
 }  // namespace yan
