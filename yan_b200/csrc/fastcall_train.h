@@ -125,25 +125,54 @@ bool number(PyObject* o, double* v) {
     return true;
 }
 
-// Values (codes) and scales of a moment; `elements` of the parameter.
-bool moment(PyObject* o, bool eight_bit, int64_t elements, int device, void** values, float** scales) {
-    if (!eight_bit) {
-        const at::Tensor* t = cuda_tensor(o);
-        if (!t || t->scalar_type() != at::kFloat || t->numel() != elements || !t->is_contiguous() || t->get_device() != device) return false;
-        *values = t->data_ptr();
-        *scales = nullptr;
+// The tensors of a list, of which there may be hundreds: the first is looked at in full, the others have to be of the same kind (dispatch
+// keys: device type, layout, subclass; element type, device).  A full look at each took 30 ns, this 8.
+class AlikeTensors {
+public:
+    explicit AlikeTensors(at::ScalarType type, int device) : type_(c10::scalarTypeToTypeMeta(type)), device_(device) {}
+
+    // Address of a contiguous tensor of `elements`; false for anything else.
+    bool take(PyObject* o, int64_t elements, void** address) {
+        if (!THPVariable_CheckExact(o)) return false;
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (!known_) {
+            const at::Tensor* first = cuda_tensor(o);
+            if (!first) return false;
+            keys_ = first->key_set();
+            known_ = true;
+        }
+        c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+        if (impl->key_set() != keys_ || impl->dtype() != type_ || impl->numel() != elements || !impl->is_contiguous()) return false;
+        if (impl->device().index() != device_ || !impl->has_storage()) return false;
+        *address = impl->mutable_data();
         return true;
     }
-    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 2) return false;
-    const at::Tensor *c = cuda_tensor(PyTuple_GET_ITEM(o, 0)), *s = cuda_tensor(PyTuple_GET_ITEM(o, 1));
-    if (!c || !s || c->scalar_type() != at::kFloat8_e4m3fn || c->numel() != elements || !c->is_contiguous() || c->get_device() != device)
-        return false;
-    if (s->scalar_type() != at::kFloat || s->numel() != ceil_div(elements, 128) || !s->is_contiguous() || s->get_device() != device)
-        return false;
-    *values = c->data_ptr();
-    *scales = s->data_ptr<float>();
-    return true;
-}
+
+private:
+    caffe2::TypeMeta type_;
+    int device_;
+    bool known_ = false;
+    c10::DispatchKeySet keys_;
+};
+
+// The values (codes) and scales of a moment.
+struct Moments {
+    AlikeTensors values, scales;
+    bool eight_bit;
+
+    Moments(bool eight_bit, int device)
+        : values(eight_bit ? at::kFloat8_e4m3fn : at::kFloat, device), scales(at::kFloat, device), eight_bit(eight_bit) {}
+    bool take(PyObject* o, int64_t elements, void** value, float** scale) {
+        *scale = nullptr;
+        if (!eight_bit) return values.take(o, elements, value);
+        void* s;
+        if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != 2 || !values.take(PyTuple_GET_ITEM(o, 0), elements, value) ||
+            !scales.take(PyTuple_GET_ITEM(o, 1), ceil_div(elements, 128), &s))
+            return false;
+        *scale = static_cast<float*>(s);
+        return true;
+    }
+};
 
 // adamw(params, grads, exp_avgs, exp_avg_sqs, weight_decay (number or list), copies or None, grad_scale or None, lr, beta1, beta2, eps, step)
 PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -172,28 +201,21 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             if (!t || t->scalar_type() != at::kFloat || t->numel() != 1 || t->get_device() != device) return code(kNotTaken);
             grad_scale = t->data_ptr<float>();
         }
-        const bool eight_bit = !THPVariable_Check(m[0]);
-        const auto param_type = first->scalar_type(), grad_type = first_grad->scalar_type();
+        const bool eight_bit = PyTuple_CheckExact(m[0]);
+        AlikeTensors params(first->scalar_type(), device), grads(first_grad->scalar_type(), device), copies(at::kBFloat16, device);
+        Moments exp_avgs(eight_bit, device), exp_avg_sqs(eight_bit, device);
         std::vector<yan_b200_adamw_tensor> table(static_cast<size_t>(count));
         for (Py_ssize_t i = 0; i < count; ++i) {
             yan_b200_adamw_tensor& t = table[static_cast<size_t>(i)];
-            const at::Tensor *tp = cuda_tensor(p[i]), *tg = cuda_tensor(g[i]);
-            if (!tp || !tg || tp->scalar_type() != param_type || tg->scalar_type() != grad_type) return code(kNotTaken);
-            if (tp->get_device() != device || tg->get_device() != device || !tp->is_contiguous() || !tg->is_contiguous()) return code(kNotTaken);
-            t.numel = tp->numel();
-            if (tg->numel() != t.numel) return code(kNotTaken);
-            t.param = tp->data_ptr();
-            t.grad = tg->data_ptr();
-            if (!moment(m[i], eight_bit, t.numel, device, &t.exp_avg, &t.exp_avg_scale) ||
-                !moment(v[i], eight_bit, t.numel, device, &t.exp_avg_sq, &t.exp_avg_sq_scale))
+            void* address;
+            if (!THPVariable_CheckExact(p[i])) return code(kNotTaken);
+            t.numel = THPVariable_Unpack(p[i]).unsafeGetTensorImpl()->numel();
+            if (!params.take(p[i], t.numel, &t.param) || !grads.take(g[i], t.numel, &address)) return code(kNotTaken);
+            t.grad = address;
+            if (!exp_avgs.take(m[i], t.numel, &t.exp_avg, &t.exp_avg_scale) || !exp_avg_sqs.take(v[i], t.numel, &t.exp_avg_sq, &t.exp_avg_sq_scale))
                 return code(kNotTaken);
             t.copy = nullptr;
-            if (c != nullptr) {
-                const at::Tensor* tc = cuda_tensor(c[i]);
-                if (!tc || tc->scalar_type() != at::kBFloat16 || tc->numel() != t.numel || !tc->is_contiguous() || tc->get_device() != device)
-                    return code(kNotTaken);
-                t.copy = tc->data_ptr();
-            }
+            if (c != nullptr && !copies.take(c[i], t.numel, &t.copy)) return code(kNotTaken);
             t.weight_decay = decay;
             if (w != nullptr && !number(w[i], &t.weight_decay)) return code(kNotTaken);
         }

@@ -62,12 +62,16 @@ __device__ __forceinline__ uint32_t quantize4(uint32_t lo, uint32_t hi, const fl
 
 }  // namespace detail
 
-// One CTA of 256 threads: 128 tokens x 128 columns of one operand.  Eight threads share a row, 16 columns each; 32 rows at a time.
+// One CTA of 256 threads: 128 tokens x 128 columns of one operand.  Eight threads share a row, 16 columns each; 32 rows at a time.  Bound by
+// HBM (3 bytes per element): 8192 x (28672 + 8192) in 139 us, 6.5 TB/s; the instance for any alignment needs more registers (205 us there).
+template <bool kAllWide>
 __global__ void __launch_bounds__(256) block_cast_tokens_kernel(const CastTokensParams p) {
     __shared__ TokenBlockTable table;
     __shared__ uint4 s_max[8][16];  // [warp][8 columns as packed bf16 magnitudes]
     __shared__ uint8_t s_scale[128];
     ptx::grid_dependency_wait();
+    // The products take the SMs as this kernel leaves them, and wait for its end before they read anything.
+    ptx::grid_dependency_launch_dependents();
     const uint32_t block = blockIdx.y, second = blockIdx.x >= p.column_tiles[0] ? 1u : 0u;
     const uint32_t tile = blockIdx.x - (second != 0 ? p.column_tiles[0] : 0u);
     const CastTokensOperand& op = p.operand[second];
@@ -89,26 +93,54 @@ __global__ void __launch_bounds__(256) block_cast_tokens_kernel(const CastTokens
         byte = in_group % 4;
     }
 
+    // The scale of a column from its largest magnitude.
+    auto take_scale = [&](uint32_t amax) {
+        const uint32_t scale = detail::scale_byte_of_amax(amax);
+        s_scale[thread] = static_cast<uint8_t>(scale);
+        const uint32_t c = tile * 128 + thread, in_tile = c % op.scale_cols;
+        if (c < op.cols)
+            op.scales[((static_cast<uint64_t>(quad) * ceil_div(op.cols, op.scale_cols) + c / op.scale_cols) * ceil_div(op.scale_cols, 128u) +
+                       in_tile / 128) * kScaleTileBytes + scale_tile_offset(in_tile % 128, byte)] = static_cast<uint8_t>(scale);
+    };
+
+    if (!kAllWide && op.wide == 0) {
+        // Any alignment: a thread has one column of 64 rows, a warp reads 64 contiguous bytes at a time.
+        const uint32_t c = thread % 128, half = thread / 128, col = tile * 128 + c;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(op.z) + static_cast<uint64_t>(row0 + half * 64) * op.ld + col;
+        uint32_t h[32], amax = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) {
+            const uint32_t r = half * 64 + 2 * i;
+            const uint32_t lo = r < rows && col < op.cols ? ptx::ld_global_u16(src + static_cast<uint64_t>(2 * i) * op.ld) : 0u;
+            const uint32_t hi = r + 1 < rows && col < op.cols ? ptx::ld_global_u16(src + static_cast<uint64_t>(2 * i + 1) * op.ld) : 0u;
+            h[i] = lo | (hi << 16);
+            amax = __vmaxu2(amax, h[i] & 0x7FFF7FFFu);
+        }
+        uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_max);
+        s_amax[thread] = max(amax & 0xFFFFu, amax >> 16);
+        __syncthreads();
+        if (thread < 128) take_scale(max(s_amax[thread], s_amax[thread + 128]));
+        __syncthreads();
+        if (col >= op.codes_ld) return;
+        const float inv = detail::inverse_of_scale(s_scale[c]);
+        uint8_t* dst = op.codes + static_cast<uint64_t>(block * 128 + half * 64) * op.codes_ld + col;
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) {
+            const uint32_t q = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(h[i] << 16) * inv, __uint_as_float(h[i] & 0xFFFF0000u) * inv),
+                                                        __NV_SATFINITE, __NV_E4M3);
+            dst[static_cast<uint64_t>(2 * i) * op.codes_ld] = static_cast<uint8_t>(q);
+            dst[static_cast<uint64_t>(2 * i + 1) * op.codes_ld] = static_cast<uint8_t>(q >> 8);
+        }
+        return;
+    }
+
     const uint32_t octet = thread % 8, first_row = thread / 8, col = tile * 128 + octet * 16;
     uint4 v[4][2];
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
         const uint32_t r = first_row + 32 * i;
         v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
-        if (r >= rows || col >= op.cols) continue;
-        const __nv_bfloat16* src = op.z + static_cast<uint64_t>(row0 + r) * op.ld + col;
-        if (op.wide != 0) {
-            ptx::ld_global_32(v[i], src);
-        } else {
-            uint16_t h[16];
-#pragma unroll
-            for (uint32_t j = 0; j < 16; ++j) h[j] = col + j < op.cols ? *reinterpret_cast<const volatile uint16_t*>(src + j) : uint16_t(0);
-            uint32_t w[8];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) w[j] = h[2 * j] | (static_cast<uint32_t>(h[2 * j + 1]) << 16);
-            v[i][0] = make_uint4(w[0], w[1], w[2], w[3]);
-            v[i][1] = make_uint4(w[4], w[5], w[6], w[7]);
-        }
+        if (r < rows && col < op.cols) ptx::ld_global_32(v[i], op.z + static_cast<uint64_t>(row0 + r) * op.ld + col);
     }
     uint32_t m[8];
 #pragma unroll
@@ -128,12 +160,7 @@ __global__ void __launch_bounds__(256) block_cast_tokens_kernel(const CastTokens
         uint32_t amax = 0;
 #pragma unroll
         for (uint32_t w = 0; w < 8; ++w) amax = max(amax, static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(s_max[w])[thread]));
-        const uint32_t scale = detail::scale_byte_of_amax(amax);
-        s_scale[thread] = static_cast<uint8_t>(scale);
-        const uint32_t c = tile * 128 + thread, in_tile = c % op.scale_cols;
-        if (c < op.cols)
-            op.scales[((static_cast<uint64_t>(quad) * ceil_div(op.cols, op.scale_cols) + c / op.scale_cols) * ceil_div(op.scale_cols, 128u) +
-                       in_tile / 128) * kScaleTileBytes + scale_tile_offset(in_tile % 128, byte)] = static_cast<uint8_t>(scale);
+        take_scale(amax);
     }
     __syncthreads();
     if (col >= op.codes_ld) return;
@@ -177,9 +204,9 @@ struct WgradParams {
 // the pair in whose stretch they begin.
 struct WgradSchedule {
     TokenBlockTable blocks;
-    uint64_t length[kMaxTokenGroups + 1];  // of all tiles in front of a group
-    uint64_t origin, rest;                 // where the shared tiles begin, and their length
-    uint32_t stretches;
+    uint32_t length[kMaxTokenGroups + 1];  // of all tiles in front of a group
+    uint32_t origin, rest;                 // where the shared tiles begin, and their length
+    uint32_t stretches, shortest, longer;  // the first `longer` stretches are one longer than `shortest`
 };
 
 // A pair of CTAs computes 256 x kCols of dW at a time, each CTA 128 rows of it: per 128 tokens it loads 128 rows of A and kCols / 2 columns of
@@ -188,7 +215,7 @@ struct WgradSchedule {
 // (whose two accumulators lie side by side, so that nothing ever waits for sums to be read), 2.12 with 224, 1.95 with single CTAs of
 // 128 x 256.
 constexpr uint32_t kWgradRows = 256;
-constexpr uint32_t kWgradMinCut = 8, kWgradMinStretch = 8;
+constexpr uint32_t kWgradMinCut = 8, kWgradMinStretch = 8, kWgradMaxStoreCost = 20;
 
 template <uint32_t kCols>
 struct WgradTile {
@@ -235,15 +262,14 @@ template <uint32_t kCols>
 __device__ __forceinline__ void build_wgrad_schedule(const WgradParams& p, WgradSchedule& s) {
     build_token_blocks(p.groups, p.max_blocks, s.blocks);
     const uint32_t lane = ptx::lane_id(), per_group = wgrad_tiles_per_group<kCols>(p);
-    uint64_t at = 0;
+    uint32_t at = 0;
     for (uint32_t first = 0; first < p.groups.num_groups; first += 32) {
         const uint32_t g = first + lane;
-        const uint64_t own = g < p.groups.num_groups
-                                 ? static_cast<uint64_t>(per_group) * wgrad_length(p, s.blocks.block[g + 1] - s.blocks.block[g]) : 0u;
-        uint64_t until = own;
+        const uint32_t own = g < p.groups.num_groups ? per_group * wgrad_length(p, s.blocks.block[g + 1] - s.blocks.block[g]) : 0u;
+        uint32_t until = own;
 #pragma unroll
         for (uint32_t off = 1; off < 32; off *= 2) {
-            const uint64_t v = __shfl_up_sync(0xffffffffu, until, off);
+            const uint32_t v = __shfl_up_sync(0xffffffffu, until, off);
             if (lane >= off) until += v;
         }
         if (g < p.groups.num_groups) s.length[g] = at + until - own;
@@ -255,9 +281,11 @@ __device__ __forceinline__ void build_wgrad_schedule(const WgradParams& p, Wgrad
         const uint32_t g = p.whole_tiles / per_group;
         s.origin = at;
         if (g < p.groups.num_groups)
-            s.origin = s.length[g] + static_cast<uint64_t>(p.whole_tiles % per_group) * wgrad_length(p, s.blocks.block[g + 1] - s.blocks.block[g]);
+            s.origin = s.length[g] + p.whole_tiles % per_group * wgrad_length(p, s.blocks.block[g + 1] - s.blocks.block[g]);
         s.rest = at - s.origin;
-        s.stretches = static_cast<uint32_t>(max(min(static_cast<uint64_t>(gridDim.x / 2), s.rest / kWgradMinStretch), static_cast<uint64_t>(1)));
+        s.stretches = max(min(gridDim.x / 2, s.rest / kWgradMinStretch), 1u);
+        s.shortest = s.rest / s.stretches;
+        s.longer = s.rest % s.stretches;
     }
 }
 
@@ -274,11 +302,11 @@ template <uint32_t kCols>
 struct WgradWalk {
     uint32_t pair, pairs;
     uint32_t tile;        // next of the dealt tiles
-    uint64_t at, end;     // what is left of the pair's stretch
+    uint32_t at, end;     // what is left of the pair's stretch
 
     __device__ __forceinline__ explicit WgradWalk(const WgradSchedule& s) : pair(blockIdx.x / 2), pairs(gridDim.x / 2), tile(blockIdx.x / 2) {
-        at = pair < s.stretches ? s.origin + pair * s.rest / s.stretches : 0u;
-        end = pair < s.stretches ? s.origin + (pair + 1u) * s.rest / s.stretches : 0u;
+        at = pair < s.stretches ? s.origin + pair * s.shortest + min(pair, s.longer) : 0u;
+        end = pair < s.stretches ? at + s.shortest + (pair < s.longer ? 1u : 0u) : 0u;
     }
 
     __device__ __forceinline__ static void place(const WgradParams& p, const WgradSchedule& s, uint32_t group, uint32_t in_group, WgradUnit& u) {
@@ -292,8 +320,9 @@ struct WgradWalk {
         u.blocks = s.blocks.block[group + 1] - u.block0;
     }
     // The pair in whose stretch a position lies.
-    __device__ __forceinline__ static uint32_t owner(const WgradSchedule& s, uint64_t position) {
-        return static_cast<uint32_t>(((position - s.origin + 1) * s.stretches - 1) / s.rest);
+    __device__ __forceinline__ static uint32_t owner(const WgradSchedule& s, uint32_t position) {
+        const uint32_t x = position - s.origin, in_longer = s.longer * (s.shortest + 1);
+        return x < in_longer ? x / (s.shortest + 1) : s.longer + (x - in_longer) / s.shortest;
     }
 
     __device__ __forceinline__ bool next(const WgradParams& p, const WgradSchedule& s, WgradUnit& u) {
@@ -313,10 +342,9 @@ struct WgradWalk {
                 else high = mid;
             }
             const uint32_t blocks = s.blocks.block[low + 1] - s.blocks.block[low], length = wgrad_length(p, blocks);
-            const uint32_t in_group = static_cast<uint32_t>((at - s.length[low]) / length);
-            const uint64_t start = s.length[low] + static_cast<uint64_t>(in_group) * length;
-            const uint32_t from = static_cast<uint32_t>(at - start);  // above zero only in the tile that the stretch begins in
-            const uint64_t until = end - start;
+            const uint32_t in_group = (at - s.length[low]) / length, start = s.length[low] + in_group * length;
+            const uint32_t from = at - start;  // above zero only in the tile that the stretch begins in
+            const uint32_t until = end - start;
             at = start + length;
             place(p, s, low, in_group, u);
             if (blocks < kWgradMinCut) {
@@ -326,7 +354,7 @@ struct WgradWalk {
                 return true;
             }
             u.begin = from >= blocks ? blocks : from & ~3u;
-            u.count = (until >= blocks ? blocks : static_cast<uint32_t>(until) & ~3u) - u.begin;
+            u.count = (until >= blocks ? blocks : until & ~3u) - u.begin;
             if (u.count == 0) continue;
             u.first_pair = owner(s, start + 3);  // a stretch that ends in the first three k-blocks has none of them
             u.last_pair = owner(s, start + blocks - 1);
@@ -469,12 +497,15 @@ __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
         ptx::fence_barrier_init();
         ptx::fence_proxy_async_smem();
     }
-    ptx::grid_dependency_wait();
-    if (warp == 3) detail::build_wgrad_schedule<kCols>(p, schedule);
+    // Up to here and for the tensor memory this kernel runs beside the cast in front of it, which lets it start when everything in front of
+    // the cast has ended.  Group sizes are known only then, too, but one group of all rows is no secret.
+    if (warp == 3 && p.groups.sizes == nullptr) detail::build_wgrad_schedule<kCols>(p, schedule);
     if (warp == 2) {
         ptx::tmem_alloc_pair(tmem_slot, T::kTmemCols);
         ptx::tmem_relinquish_alloc_permit_pair();
     }
+    ptx::grid_dependency_wait();
+    if (warp == 3 && p.groups.sizes != nullptr) detail::build_wgrad_schedule<kCols>(p, schedule);
     ptx::tcgen05_fence_before_thread_sync();
     __syncthreads();
     ptx::cluster_arrive(), ptx::cluster_wait();  // the other CTA's barriers and tensor memory are ready
@@ -616,7 +647,7 @@ __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
                     if (last || (T::kShared != 0 && c + 16 == T::kShared)) {
                         ptx::tcgen05_fence_before_thread_sync();
                         __syncwarp();
-                        if (lane == 0 && (last || (buf == 0) == (part >= 4))) ptx::mbar_arrive_cluster((last ? empty_of_pair : shared_of_pair) + buf * 8);
+                        if (lane == 0 && (last || (buf == 0) == (part >= 4))) ptx::mbar_arrive_cluster_relaxed((last ? empty_of_pair : shared_of_pair) + buf * 8);
                     }
 #pragma unroll
                     for (uint32_t j = 0; j < 16; ++j) acc[c + j] += __uint_as_float(t[j]);
@@ -714,6 +745,8 @@ inline bool plan_wgrad_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t
     const uint64_t tiles = static_cast<uint64_t>(ceil_div(n, kWgradRows)) * ceil_div(k, w.cols) * groups;
     if (tiles > 0x7fffffffull || static_cast<uint64_t>(w.blocks) * 128 > 0x7fffffffull || num_sms == 0) return false;
     w.tiles = static_cast<uint32_t>(tiles);
+    // the length of all tiles (WgradSchedule) is counted in 32 bits
+    if (tiles / groups * (w.blocks + static_cast<uint64_t>(groups) * kWgradMaxStoreCost) > 0xffffffffull) return false;
     // a pair per tile, or per kWgradMinCut k-blocks of one
     const uint64_t useful = tiles * (1 + w.blocks / kWgradMinCut), pairs = num_sms > 1 ? num_sms / 2 : 1;
     w.pairs = static_cast<uint32_t>(useful < pairs ? useful : pairs);
@@ -830,7 +863,8 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
         cfg.stream = stream;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        if (cudaLaunchKernelEx(&cfg, block_cast_tokens_kernel, c) != cudaSuccess) {
+        const bool wide = c.operand[0].wide != 0 && c.operand[1].wide != 0;
+        if (cudaLaunchKernelEx(&cfg, wide ? block_cast_tokens_kernel<true> : block_cast_tokens_kernel<false>, c) != cudaSuccess) {
             cudaGetLastError();
             return kLaunchFailed;
         }
