@@ -356,7 +356,8 @@ void yan_b200_adamw_step(const yan_b200_adamw_tensor* tensors, int num_tensors, 
  * cu_seqlens: optional int32 [sequences + 1] on the device, ascending; without it sequences = 1.  Tokens outside of every sequence do
  * not count; a sequence without tokens adds nothing.  loss: one fp32; counts int32 [sequences, experts]; grad: optional, of the
  * logits' type, zero for tokens that do not count.  experts <= 1024.
- * workspace: yan_b200_moe_balance_loss_workspace_bytes(...) bytes on a 256-byte boundary; its content does not matter.
+ * workspace: yan_b200_moe_balance_loss_workspace_bytes(...) bytes on a 256-byte boundary, 0 bytes (and a null pointer) for few tokens;
+ * its content does not matter.
  */
 enum { YAN_B200_SOFTMAX = 0, YAN_B200_SIGMOID = 1 };
 size_t yan_b200_moe_balance_loss_workspace_bytes(int tokens, int experts, int sequences, int with_grad, int num_sms);

@@ -68,7 +68,7 @@ def test_adamw_of_nothing():
     assert _adamw(numel=0) == 0
 
 
-def _balance(logits=P, ids=P, mask=None, cu=None, loss=P, counts=P, grad=P, t=64, e=32, top=2, s=1, ld=32, grad_ld=32, dtype=0, ids_64=1, score=0,
+def _balance(logits=P, ids=P, mask=None, cu=None, loss=P, counts=P, grad=P, t=200000, e=32, top=2, s=1, ld=32, grad_ld=32, dtype=0, ids_64=1, score=0,
              ws=P, ws_bytes=1 << 40, sms=148):
     return _rc("yan_b200_moe_balance_loss", logits, ids, mask, cu, loss, counts, grad, t, e, top, s, ld, grad_ld, dtype, ids_64, score, 1.0, ws,
                ws_bytes, None, sms)
@@ -84,9 +84,10 @@ def test_balance_arguments(change):
 
 def test_balance_workspace():
     from yan_b200 import _lib
-    size = _lib.lib().yan_b200_moe_balance_loss_workspace_bytes(64, 32, 1, 1, 148)
-    assert size > 0 and _balance(ws_bytes=size - 1) == SMALL
-    assert _lib.lib().yan_b200_moe_balance_loss_workspace_bytes(64, 0, 1, 1, 148) == 0
+    size = _lib.lib().yan_b200_moe_balance_loss_workspace_bytes
+    assert size(200000, 32, 1, 1, 148) > 0 and _balance(ws_bytes=size(200000, 32, 1, 1, 148) - 1) == SMALL
+    assert size(64, 32, 1, 1, 148) == 0  # few tokens need none
+    assert size(64, 0, 1, 1, 148) == 0
 
 
 def test_python_operators_refuse_tensors_of_the_host():
@@ -136,7 +137,7 @@ def test_python_operators_refuse(cuda_lib):
                      ((logits, ids), dict(score="relu")), ((logits, ids), dict(token_mask=z(64, d=torch.uint8))),
                      ((logits, ids), dict(token_mask=z(63, d=torch.bool))), ((logits, ids), dict(cu_seqlens=i32(0, 64).long())),
                      ((logits, ids), dict(cu_seqlens=i32(0))), ((logits, ids), dict(grad=z(64, 16))), ((logits.t(), ids), {}),
-                     ((z(64, 1025, d=torch.float32), ids), {}), ((logits, ids), dict(workspace=z(8, d=torch.uint8)))]:
+                     ((z(64, 1025, d=torch.float32), ids), {}), ((z(200000, 16, d=torch.float32), z(200000, 2, d=torch.int64)), dict(workspace=z(8, d=torch.uint8)))]:
         with pytest.raises(AssertionError):
             yan_b200.moe_balance_loss(*args, **kw)
 

@@ -274,12 +274,13 @@ PyObject* balance(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         at::Tensor grad = at::empty({t, e}, options);
         const size_t need = g_train.balance_workspace_bytes(static_cast<int>(t), static_cast<int>(e), static_cast<int>(sequences), 1,
                                                             static_cast<int>(num_sms));
-        at::Tensor ws = at::empty({static_cast<int64_t>(need)}, options.dtype(at::kByte));
+        at::Tensor ws;
+        if (need != 0) ws = at::empty({static_cast<int64_t>(need)}, options.dtype(at::kByte));
         const void *plogits = logits->data_ptr(), *pids = ids->data_ptr();
         void* stream = current_stream();
         float* ploss = loss.data_ptr<float>();
         int* pcounts = counts.data_ptr<int>();
-        void *pgrad = grad.data_ptr(), *pws = ws.data_ptr();
+        void *pgrad = grad.data_ptr(), *pws = need != 0 ? ws.data_ptr() : nullptr;
         int rc = 0;
         Py_BEGIN_ALLOW_THREADS
         g_train.balance(plogits, pids, mask, cu, ploss, pcounts, pgrad, static_cast<int>(t), static_cast<int>(e), static_cast<int>(top),

@@ -174,10 +174,10 @@ YAN_EXPORT void yan_b200_moe_balance_loss(const void* logits, const void* expert
         return set_rc(return_code, yan::kBadArgument);
     if (tokens > 0 && (logits == nullptr || expert_ids == nullptr)) return set_rc(return_code, yan::kBadArgument);
     const size_t item = logits_dtype == YAN_B200_F32 ? 4 : 2;
-    if (!yan::is_aligned(logits, item) || !yan::is_aligned(grad, item) || !yan::is_aligned(expert_ids, ids_64 != 0 ? 8 : 4) ||
-        workspace == nullptr || !yan::is_aligned(workspace, 256))
+    if (!yan::is_aligned(logits, item) || !yan::is_aligned(grad, item) || !yan::is_aligned(expert_ids, ids_64 != 0 ? 8 : 4))
         return set_rc(return_code, yan::kBadArgument);
     const yan::BalanceWorkspace w = yan::plan_balance_workspace(tokens, experts, sequences, grad != nullptr, num_sms);
+    if (w.bytes != 0 && (workspace == nullptr || !yan::is_aligned(workspace, 256))) return set_rc(return_code, yan::kBadArgument);
     if (workspace_bytes < w.bytes) return set_rc(return_code, yan::kWorkspaceTooSmall);
     char* ws = static_cast<char*>(workspace);
     yan::BalanceParams p;
@@ -198,7 +198,8 @@ YAN_EXPORT void yan_b200_moe_balance_loss(const void* logits, const void* expert
     p.losses = reinterpret_cast<float*>(ws + w.losses);
     p.rows = reinterpret_cast<float2*>(ws + w.rows);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    set_rc(return_code, logits_dtype == YAN_B200_F32 ? yan::launch_balance<float>(p, st) : yan::launch_balance<__nv_bfloat16>(p, st));
+    set_rc(return_code, logits_dtype == YAN_B200_F32 ? yan::launch_balance<float>(p, w.cluster, st)
+                                                         : yan::launch_balance<__nv_bfloat16>(p, w.cluster, st));
 }
 
 }  // extern "C"

@@ -4,8 +4,8 @@
 //     c[s, e] = selections of e,  P[s, e] = sum over t of p[t, e],  a[s, e] = coef / S * E / (k n_s^2) * c[s, e]
 //     loss = sum over s, e of a[s, e] * P[s, e]
 //     softmax: dz_j = p_j (a_j - sum over e of a_e p_e);  sigmoid: dz_j = s_j (1 - s_j) / sum(s) * (a_j - sum over e of a_e p_e)
-// Three launches: sums over strips of tokens, the sums of the strips with a and the loss, the gradient.  No sum depends on the order
-// in which anything runs.
+// Few tokens: one launch of one cluster of CTAs, whose sums meet in distributed shared memory.  Many: three launches, sums over strips of
+// tokens, the sums of the strips with a and the loss, the gradient.  No sum depends on the order in which anything runs.
 //
 // A strip is a fixed range of tokens; it may touch several sequences, and the sums of (strip, sequence) go to slot strip + sequence:
 // both grow along the tokens, so that no two pairs share a slot and those of one sequence follow one another.
@@ -71,12 +71,14 @@ __device__ __forceinline__ uint32_t first_sequence_behind(const BalanceParams& p
     return low;
 }
 
-// How the experts of a row lie over the lanes: kLanes lanes per row, kIter times kVec neighbouring experts each.  A warp has kRows rows
-// per group of lanes in flight, so that neither the loads nor the sums over the lanes are waited for one row at a time.
+// How the experts of a row lie over the lanes: kLanes lanes per row, kIter times kVec neighbouring experts each.  A warp works on
+// kRows rows per group of lanes at a time, while as many are on their way.  What bounds it is the number of instructions beside the loads:
+// 150 for a row of 256 experts in either pass (131072 x 256: 32 us for the sums, 4.4 TB/s, and 42 us for the gradient, 5.1 TB/s; one row
+// at a time, not fetched ahead, 63 and 62).
 template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
 struct BalanceRow {
     static constexpr uint32_t kPerLane = kVec * kIter, kGroups = 32 / kLanes;
-    static constexpr uint32_t kRows = kPerLane <= 8 ? 4 : kPerLane <= 16 ? 2 : 1, kRowsPerWarp = kGroups * kRows;
+        static constexpr uint32_t kRows = kPerLane <= 8 ? 2 : 1, kRowsPerWarp = kGroups * kRows;
 
     __device__ __forceinline__ static uint32_t column(uint32_t lane, uint32_t c) {
         return (c / kVec * kLanes + lane % kLanes) * kVec + c % kVec;
@@ -132,6 +134,11 @@ struct BalanceRow {
         return v;
     }
     __device__ __forceinline__ static float largest(float v) {
+        if constexpr (kLanes == 32) {
+            float r;
+            asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+            return r;
+        }
 #pragma unroll
         for (uint32_t off = kLanes / 2; off >= 1; off /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
         return v;
@@ -147,74 +154,107 @@ struct BalanceRow {
         }
     }
 
-    // Adds the probabilities of tokens [begin, end) that the warp has its turn for, and counts those that count.  rows[token]: what
-    // their gradient needs, if there is to be one.
-    __device__ __forceinline__ static void add(const BalanceParams& p, uint32_t begin, uint32_t end, uint32_t warp, uint32_t warps, uint32_t lane,
-                                               float2* rows, float (&sums)[kPerLane], int& counted) {
-        const T* logits = static_cast<const T*>(p.logits);
-        for (uint32_t base = begin + warp * kRowsPerWarp; base < end; base += warps * kRowsPerWarp) {
-            float z[kRows][kPerLane], shift[kRows], total[kRows];
-            bool counts[kRows];
+    // Rows of one turn of a warp, on their way.
+    struct Batch {
+        float z[kRows][kPerLane];
+        bool counts[kRows];
+
+        // Tokens from `base` on, kGroups apart; those that count lie in [begin, end).
+        __device__ __forceinline__ void load(const BalanceParams& p, uint32_t base, uint32_t begin, uint32_t end, uint32_t lane) {
 #pragma unroll
             for (uint32_t r = 0; r < kRows; ++r) {
                 const uint32_t token = base + r * kGroups + lane / kLanes;
-                counts[r] = token < end && (p.mask == nullptr || p.mask[token] != 0);
-                load(logits + static_cast<uint64_t>(token) * p.logits_ld, counts[r], p.experts, lane, z[r]);
+                counts[r] = token >= begin && token < end && (p.mask == nullptr || p.mask[token] != 0);
+                BalanceRow::load(static_cast<const T*>(p.logits) + static_cast<uint64_t>(token) * p.logits_ld, counts[r], p.experts, lane, z[r]);
             }
+        }
+    };
+
+    // Takes the turns of a warp over tokens [from, end), the first to the last or backwards: the next turn's rows are fetched before this
+    // one's are worked on.
+    template <bool kBackwards, typename Work>
+    __device__ __forceinline__ static void turns(const BalanceParams& p, uint32_t from, uint32_t begin, uint32_t end, uint32_t warp, uint32_t warps,
+                                                 uint32_t lane, Work&& work) {
+        const uint32_t first = from + warp * kRowsPerWarp, step = warps * kRowsPerWarp;
+        if (first >= end) return;
+        uint32_t left = ceil_div(end - first, step);  // turns
+        uint32_t base = kBackwards ? first + (left - 1) * step : first;
+        const uint32_t onward = kBackwards ? 0u - step : step;
+        if constexpr (kPerLane > 16) {  // no registers for two
+            Batch batch;
+            for (; left != 0; --left, base += onward) {
+                batch.load(p, base, begin, end, lane);
+                work(batch, base);
+            }
+            return;
+        }
+        Batch batch[2];
+        batch[0].load(p, base, begin, end, lane);
+        for (;;) {
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                if (left > 1) batch[i ^ 1].load(p, base + onward, begin, end, lane);
+                work(batch[i], base);
+                base += onward;
+                if (--left == 0) return;
+            }
+        }
+    }
+
+    // Adds the probabilities of tokens [begin, end) that the warp has its turn for, and counts those that count.
+    // rows[token - rows_from]: what their gradient needs, if there is to be one.
+    __device__ __forceinline__ static void add(const BalanceParams& p, uint32_t begin, uint32_t end, uint32_t warp, uint32_t warps, uint32_t lane,
+                                               float2* rows, uint32_t rows_from, float (&sums)[kPerLane], int& counted) {
+        turns<false>(p, begin, begin, end, warp, warps, lane, [&](Batch& b, uint32_t base) {
+            float shift[kRows], total[kRows];
 #pragma unroll
             for (uint32_t r = 0; r < kRows; ++r) {
                 shift[r] = 0.0f;
                 if (p.sigmoid == 0) {
-                    shift[r] = z[r][0];
+                    shift[r] = b.z[r][0];
 #pragma unroll
-                    for (uint32_t c = 1; c < kPerLane; ++c) shift[r] = fmaxf(shift[r], z[r][c]);
+                    for (uint32_t c = 1; c < kPerLane; ++c) shift[r] = fmaxf(shift[r], b.z[r][c]);
                     shift[r] = largest(shift[r]);
                     if (shift[r] == -INFINITY) shift[r] = 0.0f;
                 }
             }
 #pragma unroll
             for (uint32_t r = 0; r < kRows; ++r) {
-                scores(p.sigmoid != 0, z[r], shift[r]);
+                scores(p.sigmoid != 0, b.z[r], shift[r]);
                 total[r] = 0.0f;
 #pragma unroll
-                for (uint32_t c = 0; c < kPerLane; ++c) total[r] += z[r][c];
+                for (uint32_t c = 0; c < kPerLane; ++c) total[r] += b.z[r][c];
                 total[r] = sum(total[r]);
             }
 #pragma unroll
             for (uint32_t r = 0; r < kRows; ++r) {
-                const float inverse = total[r] == 0.0f ? 0.0f : 1.0f / total[r];  // a row of nothing but -inf has zeros
+                const float inverse = total[r] == 0.0f ? 0.0f : __fdividef(1.0f, total[r]);  // a row of nothing but -inf has zeros
 #pragma unroll
-                for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = fmaf(z[r][c], inverse, sums[c]);
-                if (lane % kLanes == 0 && counts[r]) {
-                    if (rows != nullptr) rows[base + r * kGroups + lane / kLanes] = make_float2(shift[r], inverse);
+                for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = fmaf(b.z[r][c], inverse, sums[c]);
+                if (lane % kLanes == 0 && b.counts[r]) {
+                    if (rows != nullptr) rows[base + r * kGroups + lane / kLanes - rows_from] = make_float2(shift[r], inverse);
                     ++counted;
                 }
             }
-        }
+        });
     }
 
     // The gradient of tokens [at, end) that the warp has its turn for; those in front of `begin` and those that do not count have zeros.
     __device__ __forceinline__ static void grad(const BalanceParams& p, uint32_t at, uint32_t begin, uint32_t end, uint32_t warp, uint32_t warps,
-                                                uint32_t lane, const float2* rows, const float (&weights)[kPerLane]) {
-        const T* logits = static_cast<const T*>(p.logits);
+                                                uint32_t lane, const float2* rows, uint32_t rows_from, const float (&weights)[kPerLane]) {
         T* out = static_cast<T*>(p.grad);
-        for (uint32_t base = at + warp * kRowsPerWarp; base < end; base += warps * kRowsPerWarp) {
-            float z[kRows][kPerLane], inner[kRows];
+        turns<true>(p, at, begin, end, warp, warps, lane, [&](Batch& b, uint32_t base) {
+            float inner[kRows];
             float2 row[kRows];
-            bool counts[kRows];
+#pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r)
+                row[r] = b.counts[r] ? rows[base + r * kGroups + lane / kLanes - rows_from] : make_float2(0.0f, 0.0f);
 #pragma unroll
             for (uint32_t r = 0; r < kRows; ++r) {
-                const uint32_t token = base + r * kGroups + lane / kLanes;
-                counts[r] = token >= begin && token < end && (p.mask == nullptr || p.mask[token] != 0);
-                load(logits + static_cast<uint64_t>(token) * p.logits_ld, counts[r], p.experts, lane, z[r]);
-                row[r] = counts[r] ? rows[token] : make_float2(0.0f, 0.0f);
-            }
-#pragma unroll
-            for (uint32_t r = 0; r < kRows; ++r) {
-                scores(p.sigmoid != 0, z[r], row[r].x);
+                scores(p.sigmoid != 0, b.z[r], row[r].x);
                 inner[r] = 0.0f;
 #pragma unroll
-                for (uint32_t c = 0; c < kPerLane; ++c) inner[r] = fmaf(z[r][c], weights[c], inner[r]);
+                for (uint32_t c = 0; c < kPerLane; ++c) inner[r] = fmaf(b.z[r][c], weights[c], inner[r]);
                 inner[r] = sum(inner[r]);
             }
 #pragma unroll
@@ -223,12 +263,12 @@ struct BalanceRow {
                 inner[r] *= row[r].y;
 #pragma unroll
                 for (uint32_t c = 0; c < kPerLane; ++c) {
-                    const float slope = p.sigmoid != 0 ? z[r][c] * (1.0f - z[r][c]) : z[r][c];
-                    z[r][c] = counts[r] ? slope * row[r].y * (weights[c] - inner[r]) : 0.0f;
+                    const float slope = p.sigmoid != 0 ? b.z[r][c] * (1.0f - b.z[r][c]) : b.z[r][c];
+                    b.z[r][c] = b.counts[r] ? slope * row[r].y * (weights[c] - inner[r]) : 0.0f;
                 }
-                if (token < end) store(out + static_cast<uint64_t>(token) * p.grad_ld, p.experts, lane, z[r]);
+                if (token < end) store(out + static_cast<uint64_t>(token) * p.grad_ld, p.experts, lane, b.z[r]);
             }
-        }
+        });
     }
 };
 
@@ -236,13 +276,23 @@ struct BalanceRow {
 __device__ __forceinline__ void count_selections(const BalanceParams& p, uint32_t begin, uint32_t end, uint32_t thread, uint32_t threads,
                                                  int* s_counts) {
     const uint64_t first = static_cast<uint64_t>(begin) * p.top, last = static_cast<uint64_t>(end) * p.top;
-    for (uint64_t i = first + thread; i < last; i += threads) {
-        if (p.mask != nullptr) {
-            const uint32_t token = last <= 0xFFFFFFFFu ? static_cast<uint32_t>(i) / p.top : static_cast<uint32_t>(i / p.top);
-            if (p.mask[token] == 0) continue;
+    for (uint64_t at = first + thread; at < last; at += 4ull * threads) {
+        int ids[4];  // in flight together
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint64_t i = at + static_cast<uint64_t>(j) * threads;
+            ids[j] = -1;
+            if (i >= last) continue;
+            const long long id = p.ids_64 != 0 ? static_cast<const long long*>(p.ids)[i] : static_cast<const int*>(p.ids)[i];
+            if (id >= 0 && id < static_cast<long long>(p.experts)) ids[j] = static_cast<int>(id);
+            if (p.mask != nullptr) {
+                const uint32_t token = last <= 0xFFFFFFFFu ? static_cast<uint32_t>(i) / p.top : static_cast<uint32_t>(i / p.top);
+                if (p.mask[token] == 0) ids[j] = -1;
+            }
         }
-        const long long id = p.ids_64 != 0 ? static_cast<const long long*>(p.ids)[i] : static_cast<const int*>(p.ids)[i];
-        if (id >= 0 && id < static_cast<long long>(p.experts)) atomicAdd(&s_counts[id], 1);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+            if (ids[j] >= 0) atomicAdd(&s_counts[ids[j]], 1);
     }
 }
 
@@ -257,7 +307,7 @@ __device__ __forceinline__ float balance_weight(const BalanceParams& p, int coun
 }  // namespace detail
 
 template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
-__global__ void __launch_bounds__(kBalanceThreads) balance_sums_kernel(const BalanceParams p) {
+__global__ void __launch_bounds__(kBalanceThreads, kVec * kIter <= 16 ? 3 : 1) balance_sums_kernel(const BalanceParams p) {
     using Row = detail::BalanceRow<T, kVec, kLanes, kIter>;
     constexpr uint32_t kPerLane = Row::kPerLane;
     extern __shared__ float s_sums[];  // [warps][experts]
@@ -281,7 +331,7 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_sums_kernel(const Bal
 #pragma unroll
         for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = 0.0f;
         int counted = 0;
-        Row::add(p, begin, end, warp, kBalanceWarps, lane, p.grad != nullptr ? p.rows : nullptr, sums, counted);
+        Row::add(p, begin, end, warp, kBalanceWarps, lane, p.grad != nullptr ? p.rows : nullptr, 0, sums, counted);
         if (counted != 0) atomicAdd(&s_tokens, counted);
 #pragma unroll
         for (uint32_t c = 0; c < kPerLane; ++c) {
@@ -347,9 +397,9 @@ __global__ void __launch_bounds__(kBalanceWeightWarps * 32) balance_weights_kern
     if (lane == 0) p.losses[s * gridDim.x + blockIdx.x] = loss;
 }
 
-// Strips from the last to the first: what the first launch read last is what L2 still holds.
+// Strips run side by side, each from its last token to its first: what the first launch read last is what L2 still holds.
 template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
-__global__ void __launch_bounds__(kBalanceThreads) balance_grad_kernel(const BalanceParams p, uint32_t num_losses) {
+__global__ void __launch_bounds__(kBalanceThreads, kVec * kIter <= 16 ? 3 : 1) balance_grad_kernel(const BalanceParams p, uint32_t num_losses) {
     using Row = detail::BalanceRow<T, kVec, kLanes, kIter>;
     constexpr uint32_t kPerLane = Row::kPerLane;
     ptx::grid_dependency_wait();
@@ -362,7 +412,7 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_grad_kernel(const Bal
         if (lane == 0) *p.loss = loss;
     }
     if (p.grad == nullptr) return;
-    const uint32_t strip = gridDim.x - 1 - blockIdx.x, first = strip * p.strip_tokens, last = min(first + p.strip_tokens, p.tokens);
+    const uint32_t strip = blockIdx.x, first = strip * p.strip_tokens, last = min(first + p.strip_tokens, p.tokens);
     float weights[kPerLane];
     uint32_t at = first;  // tokens below have their gradient
     for (uint32_t s = detail::first_sequence_behind(p, first); at < last; ++s) {
@@ -377,8 +427,166 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_grad_kernel(const Bal
                 weights[c] = col < p.experts ? p.weights[static_cast<uint64_t>(s) * p.experts + col] : 0.0f;
             }
         }
-        Row::grad(p, at, begin, end, warp, kBalanceWarps, lane, p.rows, weights);
+        Row::grad(p, at, begin, end, warp, kBalanceWarps, lane, p.rows, 0, weights);
         at = end;
+    }
+}
+
+// ---- few tokens: one cluster ----
+// us for one cluster / for three launches: 64 x 64 6.1 / 8.2, 512 x 64 6.5 / 8.2, 512 x 256 9.4 / 9.5, 2048 x 64 10.0 / 8.7.
+constexpr uint32_t kBalanceClusterMaxLogits = 1u << 16;
+constexpr uint32_t kBalanceClusterCtas = 8, kBalanceClusterThreads = 512, kBalanceClusterWarps = kBalanceClusterThreads / 32;
+
+// Shared memory of a CTA, in words: per (sequence, expert) the sum, the selections and a; the warps' sums; per sequence its tokens; per row
+// of the CTA what its gradient needs.
+struct BalanceClusterLayout {
+    uint32_t pairs, counts, weights, warps, tokens, rows, words;
+    __host__ __device__ BalanceClusterLayout(uint32_t tokens_of_cta, uint32_t experts, uint32_t sequences) {
+        pairs = experts * sequences;
+        counts = pairs, weights = 2 * pairs, warps = 3 * pairs;
+        tokens = warps + kBalanceClusterWarps * experts;
+        rows = align_up(tokens + sequences, 2u);
+        words = rows + 2 * tokens_of_cta;
+    }
+};
+
+namespace detail {
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+// The same word of every CTA of the cluster, added up in their order.
+__device__ __forceinline__ float sum_of_cluster(const float* word) {
+    float v[kBalanceClusterCtas], sum = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kBalanceClusterCtas; ++i) v[i] = ld_cluster_f32(ptx::map_to_cta(ptx::smem_u32(word), i));
+#pragma unroll
+    for (uint32_t i = 0; i < kBalanceClusterCtas; ++i) sum += v[i];
+    return sum;
+}
+__device__ __forceinline__ int sum_of_cluster(const int* word) {
+    int sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kBalanceClusterCtas; ++i) sum += ld_cluster_s32(ptx::map_to_cta(ptx::smem_u32(word), i));
+    return sum;
+}
+
+}  // namespace detail
+
+template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
+__global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBalanceClusterCtas, 1, 1)
+    balance_cluster_kernel(const BalanceParams p, uint32_t tokens_of_cta) {
+    using Row = detail::BalanceRow<T, kVec, kLanes, kIter>;
+    constexpr uint32_t kPerLane = Row::kPerLane;
+    extern __shared__ float2 s_all[];
+    __shared__ float s_losses[kBalanceClusterCtas], s_loss[kBalanceClusterWarps];
+    const BalanceClusterLayout at(tokens_of_cta, p.experts, p.sequences);
+    float* const s_sums = reinterpret_cast<float*>(s_all);
+    int* const s_counts = reinterpret_cast<int*>(s_sums) + at.counts;
+    float* const s_weights = s_sums + at.weights;
+    float* const s_warps = s_sums + at.warps;
+    int* const s_tokens = reinterpret_cast<int*>(s_sums) + at.tokens;
+    float2* const s_rows = reinterpret_cast<float2*>(s_sums + at.rows);
+    const uint32_t thread = threadIdx.x, warp = thread / 32, lane = thread % 32, rank = ptx::cluster_ctarank();
+    const uint32_t first = min(rank * tokens_of_cta, p.tokens), last = min(first + tokens_of_cta, p.tokens);
+
+    for (uint32_t i = thread; i < 2 * at.pairs; i += kBalanceClusterThreads) s_sums[i] = 0.0f;  // and the selections
+    for (uint32_t i = thread; i < p.sequences; i += kBalanceClusterThreads) s_tokens[i] = 0;
+    __syncthreads();
+    ptx::grid_dependency_wait();
+
+    // the CTA's tokens
+    const uint32_t first_sequence = detail::first_sequence_behind(p, first);
+    for (uint32_t s = first_sequence; s < p.sequences; ++s) {
+        uint32_t begin, end;
+        detail::sequence_range(p, s, begin, end);
+        if (begin >= last) break;
+        begin = max(begin, first), end = min(end, last);
+        if (begin >= end) continue;
+        detail::count_selections(p, begin, end, thread, kBalanceClusterThreads, s_counts + s * p.experts);
+        float sums[kPerLane];
+#pragma unroll
+        for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = 0.0f;
+        int counted = 0;
+        Row::add(p, begin, end, warp, kBalanceClusterWarps, lane, p.grad != nullptr ? s_rows : nullptr, first, sums, counted);
+        if (counted != 0) atomicAdd(&s_tokens[s], counted);
+#pragma unroll
+        for (uint32_t c = 0; c < kPerLane; ++c) {
+#pragma unroll
+            for (uint32_t off = kLanes; off < 32; off *= 2) sums[c] += __shfl_xor_sync(0xffffffffu, sums[c], off);
+            const uint32_t col = Row::column(lane, c);
+            if (lane < kLanes && col < p.experts) s_warps[warp * p.experts + col] = sums[c];
+        }
+        __syncthreads();
+        for (uint32_t e = thread; e < p.experts; e += kBalanceClusterThreads) {
+            float sum = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kBalanceClusterWarps; ++w) sum += s_warps[w * p.experts + e];
+            s_sums[s * p.experts + e] = sum;
+        }
+        __syncthreads();
+    }
+    ptx::cluster_arrive(), ptx::cluster_wait();
+
+    // a of the sequences that the CTA's tokens belong to, and its share of the loss and the counts: every eighth pair
+    float loss = 0.0f;
+    for (uint32_t i = thread; i < at.pairs; i += kBalanceClusterThreads) {
+        const uint32_t s = i / p.experts;
+        uint32_t begin, end;
+        detail::sequence_range(p, s, begin, end);
+        const bool share = i % kBalanceClusterCtas == rank, mine = begin < last && end > first;
+        if (!share && !mine) continue;
+        const int count = detail::sum_of_cluster(s_counts + i);
+        const float weight = detail::balance_weight(p, count, detail::sum_of_cluster(s_tokens + s));
+        s_weights[i] = weight;
+        if (share) {
+            p.counts[i] = count;
+            loss = fmaf(weight, detail::sum_of_cluster(s_sums + i), loss);
+        }
+    }
+#pragma unroll
+    for (uint32_t off = 16; off >= 1; off /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, off);
+    if (lane == 0) s_loss[warp] = loss;
+    __syncthreads();
+    if (thread == 0) {
+        loss = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kBalanceClusterWarps; ++w) loss += s_loss[w];
+        ptx::st_cluster_f32(ptx::map_to_cta(ptx::smem_u32(s_losses + rank), 0), loss);
+    }
+    ptx::cluster_arrive();  // waited for at the end: nobody needs this CTA's memory any more, and the losses are there
+
+    if (p.grad != nullptr) {
+        float weights[kPerLane];
+        uint32_t done = first;  // tokens below have their gradient
+        for (uint32_t s = first_sequence; done < last; ++s) {
+            uint32_t begin = last, end = last;
+            if (s < p.sequences) detail::sequence_range(p, s, begin, end);
+            begin = min(max(begin, done), last), end = min(max(end, begin), last);
+            if (begin < end) {
+#pragma unroll
+                for (uint32_t c = 0; c < kPerLane; ++c) {
+                    const uint32_t col = Row::column(lane, c);
+                    weights[c] = col < p.experts ? s_weights[s * p.experts + col] : 0.0f;
+                }
+            }
+            Row::grad(p, done, begin, end, warp, kBalanceClusterWarps, lane, s_rows, first, weights);
+            done = end;
+        }
+    }
+    ptx::cluster_wait();
+    if (rank == 0 && thread == 0) {
+        loss = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kBalanceClusterCtas; ++i) loss += s_losses[i];
+        *p.loss = loss;
     }
 }
 
@@ -386,17 +594,22 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_grad_kernel(const Bal
 // host side
 // ---------------------------------------------------------------------------------------------
 struct BalanceWorkspace {
-    uint32_t strips, strip_tokens;
+    bool cluster;                  // one cluster does it, without scratch
+    uint32_t strips, strip_tokens;  // tokens of a CTA in either case
     size_t sums, counts, tokens, weights, losses, rows, bytes;
 };
 
 inline BalanceWorkspace plan_balance_workspace(uint32_t tokens, uint32_t experts, uint32_t sequences, bool with_grad, uint32_t num_sms) {
-    BalanceWorkspace w;
-#ifndef BS
-#define BS 3
-#endif
-    // two CTAs per SM, at least four tokens per warp
-    w.strip_tokens = ceil_div(tokens, BS * num_sms);
+    BalanceWorkspace w = {};
+    w.cluster = num_sms >= kBalanceClusterCtas && static_cast<uint64_t>(tokens) * experts <= kBalanceClusterMaxLogits;
+    if (w.cluster) {
+        w.strip_tokens = ceil_div(tokens, kBalanceClusterCtas);
+        w.cluster = static_cast<uint64_t>(experts) * sequences <= 16384 &&
+                    BalanceClusterLayout(w.strip_tokens, experts, sequences).words * 4 <= 200 * 1024;
+        if (w.cluster) return w;
+    }
+    // three CTAs per SM, as many as run at a time, but at least four tokens per warp
+    w.strip_tokens = ceil_div(tokens, 3 * num_sms);
     if (w.strip_tokens < 4 * kBalanceWarps) w.strip_tokens = 4 * kBalanceWarps;
     w.strips = ceil_div(tokens, w.strip_tokens);
     if (w.strips == 0) w.strips = 1;
@@ -418,11 +631,27 @@ inline BalanceWorkspace plan_balance_workspace(uint32_t tokens, uint32_t experts
 }
 
 template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
-inline int launch_balance_as(const BalanceParams& p, cudaStream_t stream) {
+inline int launch_balance_as(const BalanceParams& p, bool cluster, cudaStream_t stream) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
+    if (cluster) {
+        cfg.gridDim = dim3(kBalanceClusterCtas);
+        cfg.blockDim = dim3(kBalanceClusterThreads);
+        cfg.dynamicSmemBytes = BalanceClusterLayout(p.strip_tokens, p.experts, p.sequences).words * 4;
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        auto kernel = balance_cluster_kernel<T, kVec, kLanes, kIter>;
+        cudaError_t e = cudaSuccess;
+        if (cfg.dynamicSmemBytes > 40 * 1024)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(cfg.dynamicSmemBytes));
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, p, p.strip_tokens);
+        if (e == cudaSuccess) return kOk;
+        cudaGetLastError();
+        return kLaunchFailed;
+    }
     cfg.gridDim = dim3(p.strips);
     cfg.blockDim = dim3(kBalanceThreads);
     cfg.dynamicSmemBytes = kBalanceWarps * p.experts * sizeof(float);
@@ -446,22 +675,22 @@ inline int launch_balance_as(const BalanceParams& p, cudaStream_t stream) {
 }
 
 template <typename T>
-inline int launch_balance(const BalanceParams& p, cudaStream_t stream) {
+inline int launch_balance(const BalanceParams& p, bool cluster, cudaStream_t stream) {
     constexpr uint32_t kVec = 16 / sizeof(T);
     const bool vector = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && reinterpret_cast<uintptr_t>(p.grad) % 16 == 0 &&
                         p.logits_ld % kVec == 0 && p.grad_ld % kVec == 0 && p.experts % kVec == 0;
     if (vector) {
         const uint32_t lanes = p.experts / kVec;
-        if (lanes <= 8) return launch_balance_as<T, kVec, 8, 1>(p, stream);
-        if (lanes <= 16) return launch_balance_as<T, kVec, 16, 1>(p, stream);
-        if (lanes <= 32) return launch_balance_as<T, kVec, 32, 1>(p, stream);
-        if (lanes <= 64) return launch_balance_as<T, kVec, 32, 2>(p, stream);
-        if (lanes <= 128) return launch_balance_as<T, kVec, 32, 4>(p, stream);
-        return launch_balance_as<T, kVec, 32, 1024 / kVec / 32>(p, stream);
+        if (lanes <= 8) return launch_balance_as<T, kVec, 8, 1>(p, cluster, stream);
+        if (lanes <= 16) return launch_balance_as<T, kVec, 16, 1>(p, cluster, stream);
+        if (lanes <= 32) return launch_balance_as<T, kVec, 32, 1>(p, cluster, stream);
+        if (lanes <= 64) return launch_balance_as<T, kVec, 32, 2>(p, cluster, stream);
+        if (lanes <= 128) return launch_balance_as<T, kVec, 32, 4>(p, cluster, stream);
+        return launch_balance_as<T, kVec, 32, 1024 / kVec / 32>(p, cluster, stream);
     }
-    if (p.experts <= 64) return launch_balance_as<T, 1, 32, 2>(p, stream);
-    if (p.experts <= 256) return launch_balance_as<T, 1, 32, 8>(p, stream);
-    return launch_balance_as<T, 1, 32, 32>(p, stream);
+    if (p.experts <= 64) return launch_balance_as<T, 1, 32, 2>(p, cluster, stream);
+    if (p.experts <= 256) return launch_balance_as<T, 1, 32, 8>(p, cluster, stream);
+    return launch_balance_as<T, 1, 32, 32>(p, cluster, stream);
 }
 
 }  // namespace yan
