@@ -8,6 +8,7 @@
 //      memory.  The tensor core transposes the token-major operands and multiplies the scales in, so that nothing has to be promoted.
 
 #include <cstdint>
+#include <type_traits>
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -63,12 +64,13 @@ __device__ __forceinline__ uint32_t quantize4(uint32_t lo, uint32_t hi, const fl
 }  // namespace detail
 
 // One CTA of 256 threads: 128 tokens x 128 columns of one operand.  Eight threads share a row, 16 columns each; 32 rows at a time.  Bound by
-// HBM (3 bytes per element): 8192 x (28672 + 8192) in 139 us, 6.5 TB/s; the instance for any alignment needs more registers (205 us there).
+// HBM (3 bytes per element): 8192 x (28672 + 8192) in 139 us, 6.5 TB/s.
 template <bool kAllWide>
 __global__ void __launch_bounds__(256) block_cast_tokens_kernel(const CastTokensParams p) {
     __shared__ TokenBlockTable table;
     __shared__ uint4 s_max[8][16];  // [warp][8 columns as packed bf16 magnitudes]
     __shared__ uint8_t s_scale[128];
+    __shared__ __align__(16) uint16_t s_tile[kAllWide ? 1 : 128 * 128];
     ptx::grid_dependency_wait();
     // The products take the SMs as this kernel leaves them, and wait for its end before they read anything.
     ptx::grid_dependency_launch_dependents();
@@ -93,54 +95,29 @@ __global__ void __launch_bounds__(256) block_cast_tokens_kernel(const CastTokens
         byte = in_group % 4;
     }
 
-    // The scale of a column from its largest magnitude.
-    auto take_scale = [&](uint32_t amax) {
-        const uint32_t scale = detail::scale_byte_of_amax(amax);
-        s_scale[thread] = static_cast<uint8_t>(scale);
-        const uint32_t c = tile * 128 + thread, in_tile = c % op.scale_cols;
-        if (c < op.cols)
-            op.scales[((static_cast<uint64_t>(quad) * ceil_div(op.cols, op.scale_cols) + c / op.scale_cols) * ceil_div(op.scale_cols, 128u) +
-                       in_tile / 128) * kScaleTileBytes + scale_tile_offset(in_tile % 128, byte)] = static_cast<uint8_t>(scale);
-    };
-
-    if (!kAllWide && op.wide == 0) {
-        // Any alignment: a thread has one column of 64 rows, a warp reads 64 contiguous bytes at a time.
-        const uint32_t c = thread % 128, half = thread / 128, col = tile * 128 + c;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(op.z) + static_cast<uint64_t>(row0 + half * 64) * op.ld + col;
-        uint32_t h[32], amax = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) {
-            const uint32_t r = half * 64 + 2 * i;
-            const uint32_t lo = r < rows && col < op.cols ? ptx::ld_global_u16(src + static_cast<uint64_t>(2 * i) * op.ld) : 0u;
-            const uint32_t hi = r + 1 < rows && col < op.cols ? ptx::ld_global_u16(src + static_cast<uint64_t>(2 * i + 1) * op.ld) : 0u;
-            h[i] = lo | (hi << 16);
-            amax = __vmaxu2(amax, h[i] & 0x7FFF7FFFu);
-        }
-        uint32_t* s_amax = reinterpret_cast<uint32_t*>(s_max);
-        s_amax[thread] = max(amax & 0xFFFFu, amax >> 16);
-        __syncthreads();
-        if (thread < 128) take_scale(max(s_amax[thread], s_amax[thread + 128]));
-        __syncthreads();
-        if (col >= op.codes_ld) return;
-        const float inv = detail::inverse_of_scale(s_scale[c]);
-        uint8_t* dst = op.codes + static_cast<uint64_t>(block * 128 + half * 64) * op.codes_ld + col;
-#pragma unroll
-        for (uint32_t i = 0; i < 32; ++i) {
-            const uint32_t q = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(h[i] << 16) * inv, __uint_as_float(h[i] & 0xFFFF0000u) * inv),
-                                                        __NV_SATFINITE, __NV_E4M3);
-            dst[static_cast<uint64_t>(2 * i) * op.codes_ld] = static_cast<uint8_t>(q);
-            dst[static_cast<uint64_t>(2 * i + 1) * op.codes_ld] = static_cast<uint8_t>(q >> 8);
-        }
-        return;
-    }
-
     const uint32_t octet = thread % 8, first_row = thread / 8, col = tile * 128 + octet * 16;
     uint4 v[4][2];
+    if (kAllWide || op.wide != 0) {
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t r = first_row + 32 * i;
-        v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
-        if (r < rows && col < op.cols) ptx::ld_global_32(v[i], op.z + static_cast<uint64_t>(row0 + r) * op.ld + col);
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t r = first_row + 32 * i;
+            v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
+            if (r < rows && col < op.cols) ptx::ld_global_32(v[i], op.z + static_cast<uint64_t>(row0 + r) * op.ld + col);
+        }
+    } else if constexpr (!kAllWide) {
+        // Any alignment: an element per lane, through shared memory.
+        const uint32_t c = thread % 128, column = tile * 128 + c, there = column < op.cols ? rows : 0u;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(op.z) + static_cast<uint64_t>(row0 + thread / 128) * op.ld + column;
+#pragma unroll 16
+        for (uint32_t r = thread / 128; r < 128; r += 2, src += 2 * op.ld)
+            s_tile[r * 128 + c] = r < there ? static_cast<uint16_t>(ptx::ld_global_u16(src)) : uint16_t(0);
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint4* from = reinterpret_cast<const uint4*>(s_tile + (first_row + 32 * i) * 128 + octet * 16);
+            v[i][0] = from[0];
+            v[i][1] = from[1];
+        }
     }
     uint32_t m[8];
 #pragma unroll
@@ -160,7 +137,11 @@ __global__ void __launch_bounds__(256) block_cast_tokens_kernel(const CastTokens
         uint32_t amax = 0;
 #pragma unroll
         for (uint32_t w = 0; w < 8; ++w) amax = max(amax, static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(s_max[w])[thread]));
-        take_scale(amax);
+        const uint32_t scale = detail::scale_byte_of_amax(amax), c = tile * 128 + thread, in_tile = c % op.scale_cols;
+        s_scale[thread] = static_cast<uint8_t>(scale);
+        if (c < op.cols)
+            op.scales[((static_cast<uint64_t>(quad) * ceil_div(op.cols, op.scale_cols) + c / op.scale_cols) * ceil_div(op.scale_cols, 128u) +
+                       in_tile / 128) * kScaleTileBytes + scale_tile_offset(in_tile % 128, byte)] = static_cast<uint8_t>(scale);
     }
     __syncthreads();
     if (col >= op.codes_ld) return;
@@ -188,7 +169,6 @@ struct WgradParams {
     void* out = nullptr;                  // [groups][n][out_ld]
     uint64_t out_ld = 0, out_group = 0;   // elements
     uint32_t accumulate = 0;
-    uint32_t vector_store = 0;            // rows of dW allow four elements at a time
     uint32_t tiles = 0, whole_tiles = 0;  // all of them; those that are dealt out one by one (see WgradSchedule)
     uint32_t store_cost = 0;              // k-blocks that take as long as storing a tile
     float4* partials = nullptr;           // [2 * pairs][2 CTAs][8 warps][columns of a warp / 4][32 lanes]
@@ -215,7 +195,10 @@ struct WgradSchedule {
 // (whose two accumulators lie side by side, so that nothing ever waits for sums to be read), 2.12 with 224, 1.95 with single CTAs of
 // 128 x 256.
 constexpr uint32_t kWgradRows = 256;
-constexpr uint32_t kWgradMinCut = 8, kWgradMinStretch = 8, kWgradMaxStoreCost = 20;
+// Parts of a tile that meet in L2 cost about as much as twelve k-blocks (us with the shortest tile that is cut and the shortest stretch at
+// 8 and 8, 24 and 12, 32 and 16 k-blocks: 2048 tokens N=1024 K=512 18.5, 14.8, 14.8; 3888 tokens N=K=128 16.8, 16.1, 14.9; 4096
+// tokens N=K=4000 83.6, 84.2, 78.7).
+constexpr uint32_t kWgradMinCut = 32, kWgradMinStretch = 16, kWgradMaxStoreCost = 20;
 
 template <uint32_t kCols>
 struct WgradTile {
@@ -228,7 +211,7 @@ struct WgradTile {
     static constexpr uint32_t kScaleTiles = 1 + ceil_div(kCols, 128u);
     static constexpr uint32_t kStageScales = kScaleTiles * kScaleTileBytes;
     static constexpr uint32_t kOffA = 0, kOffB = kOffA + kStages * kStageA, kOffScales = kOffB + kStages * kStageB;
-    static constexpr uint32_t kBoxRowBytes = 64, kBoxBytes = 32 * kBoxRowBytes;  // output staging, one box per warp
+    static constexpr uint32_t kBoxBytes = 16 * 128;  // output staging, one box per warp
     static constexpr uint32_t kOffStore = kOffScales + kStages * kStageScales;
     static constexpr uint32_t kOffSchedule = kOffStore + 8 * kBoxBytes;
     static constexpr uint32_t kOffBarriers = align_up(kOffSchedule + static_cast<uint32_t>(sizeof(WgradSchedule)), 8u);
@@ -301,20 +284,22 @@ struct WgradUnit {
 template <uint32_t kCols>
 struct WgradWalk {
     uint32_t pair, pairs;
-    uint32_t tile;        // next of the dealt tiles
-    uint32_t at, end;     // what is left of the pair's stretch
+    uint32_t tile, group, in_group;  // next of the dealt tiles: its number, its group and its number there
+    uint32_t at, end;                // what is left of the pair's stretch
 
-    __device__ __forceinline__ explicit WgradWalk(const WgradSchedule& s) : pair(blockIdx.x / 2), pairs(gridDim.x / 2), tile(blockIdx.x / 2) {
+    __device__ __forceinline__ explicit WgradWalk(const WgradSchedule& s)
+        : pair(blockIdx.x / 2), pairs(gridDim.x / 2), tile(blockIdx.x / 2), group(0), in_group(blockIdx.x / 2) {
         at = pair < s.stretches ? s.origin + pair * s.shortest + min(pair, s.longer) : 0u;
         end = pair < s.stretches ? at + s.shortest + (pair < s.longer ? 1u : 0u) : 0u;
     }
 
     __device__ __forceinline__ static void place(const WgradParams& p, const WgradSchedule& s, uint32_t group, uint32_t in_group, WgradUnit& u) {
         const uint32_t tiles_n = ceil_div(p.n, kWgradRows), tiles_k = ceil_div(p.k, kCols);
-        const uint32_t band = in_group / (8 * tiles_k), in_band = in_group % (8 * tiles_k), rows = min(8u, tiles_n - band * 8);
+        const uint32_t band = in_group / (8 * tiles_k), in_band = in_group - band * (8 * tiles_k), rows = min(8u, tiles_n - band * 8);
+        const uint32_t column = rows == 8 ? in_band / 8 : in_band / rows;
         u.group = group;
-        u.row0 = (band * 8 + in_band % rows) * kWgradRows;
-        u.col0 = in_band / rows * kCols;
+        u.row0 = (band * 8 + in_band - column * rows) * kWgradRows;
+        u.col0 = column * kCols;
         u.block0 = s.blocks.block[group];
         u.quad0 = s.blocks.quad[group];
         u.blocks = s.blocks.block[group + 1] - u.block0;
@@ -328,10 +313,12 @@ struct WgradWalk {
     __device__ __forceinline__ bool next(const WgradParams& p, const WgradSchedule& s, WgradUnit& u) {
         const uint32_t per_group = wgrad_tiles_per_group<kCols>(p);
         if (tile < p.whole_tiles) {
-            place(p, s, tile / per_group, tile % per_group, u);
+            while (in_group >= per_group) in_group -= per_group, ++group;
+            place(p, s, group, in_group, u);
             u.begin = 0, u.count = u.blocks;
             u.first_pair = u.last_pair = pair;
             tile += pairs;
+            in_group += pairs;
             return true;
         }
         while (at < end) {
@@ -370,84 +357,84 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 
 __device__ __forceinline__ void red_add(float* p, float v) { asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory"); }
-__device__ __forceinline__ void red_add4(float* p, const uint4& v) {
-    asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(__uint_as_float(v.x)), "f"(__uint_as_float(v.y)),
-                 "f"(__uint_as_float(v.z)), "f"(__uint_as_float(v.w))
-                 : "memory");
+__device__ __forceinline__ void red_add4(float* p, const float4& v) {
+    asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
-// Stores a warp's 32 rows x kWarpCols columns; lane r holds row r, acc[c] column first_col + c / 16 * 16 * direction + c % 16.  The rows go through the warp's box in shared memory, 16 columns at a time in
-// fp32, so that a store instruction covers eight pieces of 64 contiguous bytes.  fp32 is added to what dW holds where dW lies, in L2:
-// every element once, so that the order does not matter, and nothing waits for the old value.  That is what bounds an accumulated tile
-// with few tokens: L2 adds 2.2 TB/s (16 experts N=4096 K=2048, 16384 tokens: 240 us; loads and stores at the end of a tile 535, loads of
-// the next tile's old values ahead of its products, from L2 as a prefetch left them, 372).  bf16 is loaded, added in 32 bits and
-// rounded once.
-template <typename out_t, uint32_t kWarpCols>
+// Stores a warp's 32 rows x kWarpCols columns; lane r holds row r, acc[c] column first_col + c / 16 * 16 * direction + c % 16.  They go
+// through the warp's box in shared memory, 16 rows x 32 columns in fp32 at a time, so that a store instruction covers four pieces of 128
+// contiguous bytes (kVector; otherwise one, an element per lane).  16-byte chunk j of box row r is at chunk j ^ r % 8.
+// What bounds it is the number of pieces: an SM sends one in two cycles, whatever its size (pieces of 64 bytes: 6400 cycles for the 128 x 256
+// of a CTA).
+// fp32 is added to what dW holds where dW lies, in L2: every element once, so that the order does not matter, and nothing waits for the
+// old value (16 experts N=4096 K=2048, 16384 tokens: loads and stores at the end of a tile took twice as long, loads of the next
+// tile's old values ahead of its products 1.5 times).  bf16 is loaded, added in 32 bits and rounded once.
+template <typename out_t, uint32_t kWarpCols, bool kVector>
 __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const WgradUnit& u, uint32_t box, uint32_t row_in_tile, uint32_t first_col,
                                                  uint32_t direction, uint32_t lane, const float (&acc)[kWarpCols]) {
-    out_t* out = reinterpret_cast<out_t*>(p.out) + u.group * p.out_group;
+    static_assert(kWarpCols % 32 == 0);
     const uint32_t row0 = u.row0 + row_in_tile;
     if (row0 >= p.n) return;
+    const uint32_t rows = min(p.n - row0, 32u);
+    // the leftmost of 32 columns, and where its pieces meet this lane: column lane_col of rows lane_row + kRowStep i
+    constexpr uint32_t kRowStep = kVector ? 4 : 1;
+    const uint32_t lane_row = kVector ? lane / 8 : 0u, lane_col = kVector ? lane % 8 * 4 : lane;
+    uint32_t col = u.col0 + (direction == 1 ? first_col : first_col - 16) + lane_col;
+    const uint32_t half = direction == 1 ? 0u : 4u;  // downwards the first 16 values are the right half
+    const uint32_t write = box + lane % 16 * 128;
+    out_t* dst = reinterpret_cast<out_t*>(p.out) + u.group * p.out_group + static_cast<uint64_t>(row0 + lane_row) * p.out_ld + col;
+    const uint64_t step = kRowStep * p.out_ld;
+    const bool accumulate = p.accumulate != 0;
 #pragma unroll
-    for (uint32_t pass = 0; pass < kWarpCols / 16; ++pass) {
-        const uint32_t col0 = u.col0 + first_col + pass * 16 * direction, chunk = lane % 4, col = col0 + chunk * 4;
-        if (col0 >= p.k) continue;
-        [[maybe_unused]] uint2 old[4];
-        if constexpr (sizeof(out_t) == 2) {
-            if (p.vector_store != 0 && p.accumulate != 0) {
+    for (uint32_t pass = 0; pass < kWarpCols / 32; ++pass) {
+        out_t* to = dst;
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t r = row0 + i * 8 + lane / 4;
-                    old[i] = make_uint2(0, 0);
-                    if (r < p.n && col < p.k) old[i] = *reinterpret_cast<const uint2*>(out + static_cast<uint64_t>(r) * p.out_ld + col);
+        for (uint32_t rows16 = 0; rows16 < 2; ++rows16) {
+            __syncwarp();  // the read-back in front is over
+            if (lane / 16 == rows16) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    const float* a = acc + pass * 32 + j * 4;
+                    ptx::st_shared_v4(write + (((j ^ half) ^ (lane % 8)) << 4),
+                                      make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3])));
                 }
             }
-        }
-        __syncwarp();  // the read-back of the previous pass is over
+            __syncwarp();
+            const uint32_t there = col < p.k && rows > rows16 * 16 ? rows - rows16 * 16 : 0u;  // rows
+            if constexpr (kVector) {
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const float* a = acc + pass * 16 + j * 4;
-            ptx::st_shared_v4(box + lane * 64 + ((j ^ ((lane >> 1) & 3u)) << 4),
-                              make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3])));
-        }
-        __syncwarp();
-        if (p.vector_store != 0) {
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t r = i * 8 + lane / 4;
-                uint4 v = ptx::ld_shared_v4(box + r * 64 + ((chunk ^ ((r >> 1) & 3u)) << 4));
-                if (row0 + r >= p.n || col >= p.k) continue;
-                out_t* dst = out + static_cast<uint64_t>(row0 + r) * p.out_ld + col;
-                if constexpr (sizeof(out_t) == 4) {
-                    if (p.accumulate != 0) red_add4(dst, v);
-                    else *reinterpret_cast<uint4*>(dst) = v;
-                } else {
-                    if (p.accumulate != 0) {
-                        v.x = __float_as_uint(__uint_as_float(v.x) + __uint_as_float(old[i].x << 16));
-                        v.y = __float_as_uint(__uint_as_float(v.y) + __uint_as_float(old[i].x & 0xFFFF0000u));
-                        v.z = __float_as_uint(__uint_as_float(v.z) + __uint_as_float(old[i].y << 16));
-                        v.w = __float_as_uint(__uint_as_float(v.w) + __uint_as_float(old[i].y & 0xFFFF0000u));
+                for (uint32_t i = 0; i < 4; ++i, to += step) {
+                    const uint32_t r = i * 4 + lane_row;
+                    float4 v = ptx::ld_shared_v4_f32(box + r * 128 + ((lane % 8 ^ (r & 7u)) << 4));
+                    if (r >= there) continue;
+                    if constexpr (sizeof(out_t) == 4) {
+                        if (accumulate) red_add4(to, v);
+                        else *reinterpret_cast<float4*>(to) = v;
+                    } else {
+                        if (accumulate) {
+                            const uint2 old = *reinterpret_cast<const uint2*>(to);
+                            v.x += __uint_as_float(old.x << 16), v.y += __uint_as_float(old.x & 0xFFFF0000u);
+                            v.z += __uint_as_float(old.y << 16), v.w += __uint_as_float(old.y & 0xFFFF0000u);
+                        }
+                        *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
                     }
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(__uint_as_float(v.x), __uint_as_float(v.y)),
-                                                                pack_bf16(__uint_as_float(v.z), __uint_as_float(v.w)));
                 }
-            }
-        } else {
-            // one element per lane, two rows at a time
-            const uint32_t c = lane % 16, column = col0 + c;
+            } else {
 #pragma unroll 4
-            for (uint32_t r = lane / 16; r < 32; r += 2) {
-                const float v = ptx::ld_shared_f32(box + r * 64 + (((c / 4) ^ ((r >> 1) & 3u)) << 4) + c % 4 * 4);
-                if (row0 + r >= p.n || column >= p.k) continue;
-                out_t* dst = out + static_cast<uint64_t>(row0 + r) * p.out_ld + column;
-                if constexpr (sizeof(out_t) == 4) {
-                    if (p.accumulate != 0) red_add(dst, v);
-                    else *dst = v;
-                } else {
-                    *dst = __float2bfloat16_rn(p.accumulate != 0 ? v + __bfloat162float(*dst) : v);
+                for (uint32_t r = 0; r < 16; ++r, to += step) {
+                    const float v = ptx::ld_shared_f32(box + r * 128 + (((lane / 4) ^ (r & 7u)) << 4) + lane % 4 * 4);
+                    if (r >= there) continue;
+                    if constexpr (sizeof(out_t) == 4) {
+                        if (accumulate) red_add(to, v);
+                        else *to = v;
+                    } else {
+                        *to = __float2bfloat16_rn(accumulate ? v + __bfloat162float(*to) : v);
+                    }
                 }
             }
         }
+        col += 32 * direction;
+        dst += static_cast<int>(32 * direction);
     }
 }
 
@@ -458,7 +445,7 @@ struct WgradMaps {
     CUtensorMap scales_n, scales_k;  // their scale tiles: a box is what a tile of products needs
 };
 
-template <uint32_t kCols, typename out_t>
+template <uint32_t kCols, typename out_t, bool kVector>
 __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
     fp8_wgrad_kernel(const WgradParams p, const __grid_constant__ WgradMaps maps) {
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
@@ -686,7 +673,7 @@ __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
             } else if (u.blocks == 0 && p.accumulate != 0) {
                 continue;
             }
-            detail::store_wgrad_rows<out_t, kWarpCols>(p, u, box, rank * 128 + quarter * 32, first_col, direction, lane, acc);
+            detail::store_wgrad_rows<out_t, kWarpCols, kVector>(p, u, box, rank * 128 + quarter * 32, first_col, direction, lane, acc);
         }
         __syncwarp();
     }
@@ -785,7 +772,7 @@ inline CUtensorMap make_scale_tiles_desc(const void* base, uint64_t tiles, uint3
     return map;
 }
 
-template <uint32_t kCols, typename out_t>
+template <uint32_t kCols, typename out_t, bool kVector>
 inline int launch_wgrad_products(const WgradParams& p, const WgradMaps& maps, uint32_t pairs, cudaStream_t stream) {
     constexpr uint32_t kSmem = WgradTile<kCols>::kSmemSize;
     int device = 0, max_smem = 0;
@@ -802,7 +789,7 @@ inline int launch_wgrad_products(const WgradParams& p, const WgradMaps& maps, ui
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    auto kernel = fp8_wgrad_kernel<kCols, out_t>;
+    auto kernel = fp8_wgrad_kernel<kCols, out_t, kVector>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)) != cudaSuccess ||
         cudaLaunchKernelEx(&cfg, kernel, p, maps) != cudaSuccess) {
         cudaGetLastError();
@@ -877,7 +864,7 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
     p.out = a.out, p.out_ld = a.out_ld, p.out_group = a.out_group;
     p.accumulate = a.accumulate;
     const uint32_t vec = 4, item = a.out_bf16 ? 2 : 4;  // four columns at a time
-    p.vector_store = is_aligned(a.out, vec * item) && a.out_ld % vec == 0 && a.out_group % vec == 0 && a.k % vec == 0;
+    const bool vector = is_aligned(a.out, vec * item) && a.out_ld % vec == 0 && a.out_group % vec == 0 && a.k % vec == 0;
     p.tiles = w.tiles, p.whole_tiles = w.whole_tiles;
     // A CTA's 128 rows of a tile, about 100 KB in fp32, leave at 1/148 of the memory's rate in the time of about ten k-blocks.
     p.store_cost = (a.out_bf16 ? 5u : 10u) * (a.accumulate ? 2u : 1u);
@@ -885,9 +872,14 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
     p.counters = reinterpret_cast<uint32_t*>(ws + w.counters);
     p.status = a.status;
     p.timeout_ns = a.timeout_ns;
-    if (w.cols == 192)
-        return a.out_bf16 ? launch_wgrad_products<192, __nv_bfloat16>(p, maps, w.pairs, stream) : launch_wgrad_products<192, float>(p, maps, w.pairs, stream);
-    return a.out_bf16 ? launch_wgrad_products<256, __nv_bfloat16>(p, maps, w.pairs, stream) : launch_wgrad_products<256, float>(p, maps, w.pairs, stream);
+    auto launch = [&](auto out, auto vectors) {
+        using out_t = decltype(out);
+        constexpr bool kVector = decltype(vectors)::value;
+        return w.cols == 192 ? launch_wgrad_products<192, out_t, kVector>(p, maps, w.pairs, stream)
+                             : launch_wgrad_products<256, out_t, kVector>(p, maps, w.pairs, stream);
+    };
+    if (a.out_bf16) return vector ? launch(__nv_bfloat16(), std::true_type()) : launch(__nv_bfloat16(), std::false_type());
+    return vector ? launch(float(), std::true_type()) : launch(float(), std::false_type());
 }
 
 }  // namespace yan

@@ -48,24 +48,34 @@ struct BalanceParams {
 
 namespace detail {
 
+// The ends of the sequences in shared memory, as far as they fit: every kernel searches and walks them, and each look at global memory
+// would be a round trip to L2.  Ends with a barrier of the CTA; null without sequences.
+constexpr uint32_t kMaxSharedSequences = 1024;
+__device__ __forceinline__ const int* stage_sequences(const BalanceParams& p, int (&s_cu)[kMaxSharedSequences + 1]) {
+    if (p.cu_seqlens == nullptr || p.sequences > kMaxSharedSequences) return p.cu_seqlens;
+    for (uint32_t i = threadIdx.x; i <= p.sequences; i += blockDim.x) s_cu[i] = ptx::ld_global(p.cu_seqlens + i);
+    __syncthreads();
+    return s_cu;
+}
+
 // Tokens of sequence s that exist.
-__device__ __forceinline__ void sequence_range(const BalanceParams& p, uint32_t s, uint32_t& begin, uint32_t& end) {
-    if (p.cu_seqlens == nullptr) {
+__device__ __forceinline__ void sequence_range(const BalanceParams& p, const int* cu, uint32_t s, uint32_t& begin, uint32_t& end) {
+    if (cu == nullptr) {
         begin = 0, end = p.tokens;
         return;
     }
     const int limit = static_cast<int>(p.tokens);
-    begin = min(max(ptx::ld_global(p.cu_seqlens + s), 0), limit);
-    end = max(min(ptx::ld_global(p.cu_seqlens + s + 1), limit), static_cast<int>(begin));
+    begin = min(max(cu[s], 0), limit);
+    end = max(min(cu[s + 1], limit), static_cast<int>(begin));
 }
 
 // First sequence that ends behind `token` (sequences if there is none); ends do not decrease.
-__device__ __forceinline__ uint32_t first_sequence_behind(const BalanceParams& p, uint32_t token) {
-    if (p.cu_seqlens == nullptr) return 0;
+__device__ __forceinline__ uint32_t first_sequence_behind(const BalanceParams& p, const int* cu, uint32_t token) {
+    if (cu == nullptr) return 0;
     uint32_t low = 0, high = p.sequences;
     while (low < high) {
         const uint32_t mid = (low + high) / 2;
-        if (ptx::ld_global(p.cu_seqlens + mid + 1) > static_cast<int>(token)) high = mid;
+        if (cu[mid + 1] > static_cast<int>(token)) high = mid;
         else low = mid + 1;
     }
     return low;
@@ -138,10 +148,11 @@ struct BalanceRow {
             float r;
             asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
             return r;
-        }
+        } else {
 #pragma unroll
-        for (uint32_t off = kLanes / 2; off >= 1; off /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-        return v;
+            for (uint32_t off = kLanes / 2; off >= 1; off /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+            return v;
+        }
     }
     // z -> scores before they are divided by their sum; `shift` is the largest logit (softmax).
     __device__ __forceinline__ static void scores(bool sigmoid, float (&z)[kPerLane], float shift) {
@@ -312,14 +323,15 @@ __global__ void __launch_bounds__(kBalanceThreads, kVec * kIter <= 16 ? 3 : 1) b
     constexpr uint32_t kPerLane = Row::kPerLane;
     extern __shared__ float s_sums[];  // [warps][experts]
     __shared__ int s_counts[kMaxBalanceExperts];
-    __shared__ int s_tokens;
+    __shared__ int s_tokens, s_cu[detail::kMaxSharedSequences + 1];
     ptx::grid_dependency_wait();
     ptx::grid_dependency_launch_dependents();  // the next launch waits for the end of this one before it reads anything
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t strip = blockIdx.x, first = strip * p.strip_tokens, last = min(first + p.strip_tokens, p.tokens);
-    for (uint32_t s = detail::first_sequence_behind(p, first); s < p.sequences; ++s) {
+    const int* cu = detail::stage_sequences(p, s_cu);
+    for (uint32_t s = detail::first_sequence_behind(p, cu, first); s < p.sequences; ++s) {
         uint32_t begin, end;
-        detail::sequence_range(p, s, begin, end);
+        detail::sequence_range(p, cu, s, begin, end);
         if (begin >= last) break;
         begin = max(begin, first), end = min(end, last);
         if (begin >= end) continue;
@@ -361,9 +373,10 @@ __global__ void __launch_bounds__(kBalanceWeightWarps * 32) balance_weights_kern
     __shared__ int s_count[kBalanceWeightWarps][32], s_tokens[kBalanceWeightWarps];
     ptx::grid_dependency_wait();
     ptx::grid_dependency_launch_dependents();
+    const int* cu = p.cu_seqlens;
     const uint32_t s = blockIdx.y, lane = threadIdx.x % 32, e = blockIdx.x * 32 + lane, part = threadIdx.x / 32;
     uint32_t begin, end;
-    detail::sequence_range(p, s, begin, end);
+    detail::sequence_range(p, cu, s, begin, end);
     float sum = 0.0f;
     int count = 0, tokens = 0;
     if (begin < end) {
@@ -402,6 +415,7 @@ template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
 __global__ void __launch_bounds__(kBalanceThreads, kVec * kIter <= 16 ? 3 : 1) balance_grad_kernel(const BalanceParams p, uint32_t num_losses) {
     using Row = detail::BalanceRow<T, kVec, kLanes, kIter>;
     constexpr uint32_t kPerLane = Row::kPerLane;
+    __shared__ int s_cu[detail::kMaxSharedSequences + 1];
     ptx::grid_dependency_wait();
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (blockIdx.x == 0 && warp == 0) {
@@ -413,12 +427,13 @@ __global__ void __launch_bounds__(kBalanceThreads, kVec * kIter <= 16 ? 3 : 1) b
     }
     if (p.grad == nullptr) return;
     const uint32_t strip = blockIdx.x, first = strip * p.strip_tokens, last = min(first + p.strip_tokens, p.tokens);
+    const int* cu = detail::stage_sequences(p, s_cu);
     float weights[kPerLane];
     uint32_t at = first;  // tokens below have their gradient
-    for (uint32_t s = detail::first_sequence_behind(p, first); at < last; ++s) {
+    for (uint32_t s = detail::first_sequence_behind(p, cu, first); at < last; ++s) {
         // the tokens up to the sequence belong to none: their gradient is zero
         uint32_t begin = last, end = last;
-        if (s < p.sequences) detail::sequence_range(p, s, begin, end);
+        if (s < p.sequences) detail::sequence_range(p, cu, s, begin, end);
         begin = min(max(begin, at), last), end = min(max(end, begin), last);
         if (begin < end) {
 #pragma unroll
@@ -487,6 +502,7 @@ __global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBala
     constexpr uint32_t kPerLane = Row::kPerLane;
     extern __shared__ float2 s_all[];
     __shared__ float s_losses[kBalanceClusterCtas], s_loss[kBalanceClusterWarps];
+    __shared__ int s_cu[detail::kMaxSharedSequences + 1];
     const BalanceClusterLayout at(tokens_of_cta, p.experts, p.sequences);
     float* const s_sums = reinterpret_cast<float*>(s_all);
     int* const s_counts = reinterpret_cast<int*>(s_sums) + at.counts;
@@ -503,10 +519,11 @@ __global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBala
     ptx::grid_dependency_wait();
 
     // the CTA's tokens
-    const uint32_t first_sequence = detail::first_sequence_behind(p, first);
+    const int* cu = detail::stage_sequences(p, s_cu);
+    const uint32_t first_sequence = detail::first_sequence_behind(p, cu, first);
     for (uint32_t s = first_sequence; s < p.sequences; ++s) {
         uint32_t begin, end;
-        detail::sequence_range(p, s, begin, end);
+        detail::sequence_range(p, cu, s, begin, end);
         if (begin >= last) break;
         begin = max(begin, first), end = min(end, last);
         if (begin >= end) continue;
@@ -540,7 +557,7 @@ __global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBala
     for (uint32_t i = thread; i < at.pairs; i += kBalanceClusterThreads) {
         const uint32_t s = i / p.experts;
         uint32_t begin, end;
-        detail::sequence_range(p, s, begin, end);
+        detail::sequence_range(p, cu, s, begin, end);
         const bool share = i % kBalanceClusterCtas == rank, mine = begin < last && end > first;
         if (!share && !mine) continue;
         const int count = detail::sum_of_cluster(s_counts + i);
@@ -568,7 +585,7 @@ __global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBala
         uint32_t done = first;  // tokens below have their gradient
         for (uint32_t s = first_sequence; done < last; ++s) {
             uint32_t begin = last, end = last;
-            if (s < p.sequences) detail::sequence_range(p, s, begin, end);
+            if (s < p.sequences) detail::sequence_range(p, cu, s, begin, end);
             begin = min(max(begin, done), last), end = min(max(end, begin), last);
             if (begin < end) {
 #pragma unroll
@@ -688,8 +705,13 @@ inline int launch_balance(const BalanceParams& p, bool cluster, cudaStream_t str
         if (lanes <= 128) return launch_balance_as<T, kVec, 32, 4>(p, cluster, stream);
         return launch_balance_as<T, kVec, 32, 1024 / kVec / 32>(p, cluster, stream);
     }
+    // one expert per lane at a time: as few turns as the experts need
+    if (p.experts <= 32) return launch_balance_as<T, 1, 32, 1>(p, cluster, stream);
     if (p.experts <= 64) return launch_balance_as<T, 1, 32, 2>(p, cluster, stream);
+    if (p.experts <= 128) return launch_balance_as<T, 1, 32, 4>(p, cluster, stream);
     if (p.experts <= 256) return launch_balance_as<T, 1, 32, 8>(p, cluster, stream);
+    if (p.experts <= 384) return launch_balance_as<T, 1, 32, 12>(p, cluster, stream);
+    if (p.experts <= 512) return launch_balance_as<T, 1, 32, 16>(p, cluster, stream);
     return launch_balance_as<T, 1, 32, 32>(p, cluster, stream);
 }
 
