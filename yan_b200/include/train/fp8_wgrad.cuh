@@ -385,9 +385,20 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
     out_t* dst = reinterpret_cast<out_t*>(p.out) + u.group * p.out_group + static_cast<uint64_t>(row0 + lane_row) * p.out_ld + col;
     const uint64_t step = kRowStep * p.out_ld;
     const bool accumulate = p.accumulate != 0;
+    // bf16, vectors: the old values of a pass are fetched one pass ahead
+    constexpr bool kFetch = sizeof(out_t) == 2 && kVector;
+    [[maybe_unused]] uint2 old[kFetch ? 8 : 1], next_old[kFetch ? 8 : 1];
+    auto fetch = [&](uint2 (&into)[kFetch ? 8 : 1], const out_t* from, uint32_t at_col) {
+#pragma unroll
+        for (uint32_t i = 0; i < (kFetch ? 8 : 0); ++i)
+            if (at_col < p.k && i * 4 + lane_row < rows) into[i] = *reinterpret_cast<const uint2*>(from + i * step);
+    };
+    if (kFetch && accumulate) fetch(old, dst, col);
 #pragma unroll
     for (uint32_t pass = 0; pass < kWarpCols / 32; ++pass) {
         out_t* to = dst;
+        if (kFetch && accumulate && pass + 1 < kWarpCols / 32)
+            fetch(next_old, dst + static_cast<int>(32 * direction), col + 32 * direction);
 #pragma unroll
         for (uint32_t rows16 = 0; rows16 < 2; ++rows16) {
             __syncwarp();  // the read-back in front is over
@@ -412,9 +423,9 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
                         else *reinterpret_cast<float4*>(to) = v;
                     } else {
                         if (accumulate) {
-                            const uint2 old = *reinterpret_cast<const uint2*>(to);
-                            v.x += __uint_as_float(old.x << 16), v.y += __uint_as_float(old.x & 0xFFFF0000u);
-                            v.z += __uint_as_float(old.y << 16), v.w += __uint_as_float(old.y & 0xFFFF0000u);
+                            const uint2 o = old[rows16 * 4 + i];
+                            v.x += __uint_as_float(o.x << 16), v.y += __uint_as_float(o.x & 0xFFFF0000u);
+                            v.z += __uint_as_float(o.y << 16), v.w += __uint_as_float(o.y & 0xFFFF0000u);
                         }
                         *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
                     }
@@ -432,6 +443,10 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
                     }
                 }
             }
+        }
+        if constexpr (kFetch) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) old[i] = next_old[i];
         }
         col += 32 * direction;
         dst += static_cast<int>(32 * direction);

@@ -88,7 +88,7 @@ __device__ __forceinline__ uint32_t first_sequence_behind(const BalanceParams& p
 template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
 struct BalanceRow {
     static constexpr uint32_t kPerLane = kVec * kIter, kGroups = 32 / kLanes;
-        static constexpr uint32_t kRows = kPerLane <= 8 ? 2 : 1, kRowsPerWarp = kGroups * kRows;
+        static constexpr uint32_t kRows = kPerLane <= 2 ? 4 : kPerLane <= 8 ? 2 : 1, kRowsPerWarp = kGroups * kRows;
 
     __device__ __forceinline__ static uint32_t column(uint32_t lane, uint32_t c) {
         return (c / kVec * kLanes + lane % kLanes) * kVec + c % kVec;
@@ -452,14 +452,14 @@ __global__ void __launch_bounds__(kBalanceThreads, kVec * kIter <= 16 ? 3 : 1) b
 constexpr uint32_t kBalanceClusterMaxLogits = 1u << 16;
 constexpr uint32_t kBalanceClusterCtas = 8, kBalanceClusterThreads = 512, kBalanceClusterWarps = kBalanceClusterThreads / 32;
 
-// Shared memory of a CTA, in words: per (sequence, expert) the sum, the selections and a; the warps' sums; per sequence its tokens; per row
-// of the CTA what its gradient needs.
+// Shared memory of a CTA, in words: per (sequence, expert) the sum, the selections and a; the slots of (warp, sequence) sums; per sequence its
+// tokens; per row of the CTA what its gradient needs.
 struct BalanceClusterLayout {
-    uint32_t pairs, counts, weights, warps, tokens, rows, words;
+    uint32_t pairs, counts, weights, slots, tokens, rows, words;
     __host__ __device__ BalanceClusterLayout(uint32_t tokens_of_cta, uint32_t experts, uint32_t sequences) {
         pairs = experts * sequences;
-        counts = pairs, weights = 2 * pairs, warps = 3 * pairs;
-        tokens = warps + kBalanceClusterWarps * experts;
+        counts = pairs, weights = 2 * pairs, slots = 3 * pairs;
+        tokens = slots + (kBalanceClusterWarps + sequences) * experts;
         rows = align_up(tokens + sequences, 2u);
         words = rows + 2 * tokens_of_cta;
     }
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBala
     float* const s_sums = reinterpret_cast<float*>(s_all);
     int* const s_counts = reinterpret_cast<int*>(s_sums) + at.counts;
     float* const s_weights = s_sums + at.weights;
-    float* const s_warps = s_sums + at.warps;
+    float* const s_slots = s_sums + at.slots;
     int* const s_tokens = reinterpret_cast<int*>(s_sums) + at.tokens;
     float2* const s_rows = reinterpret_cast<float2*>(s_sums + at.rows);
     const uint32_t thread = threadIdx.x, warp = thread / 32, lane = thread % 32, rank = ptx::cluster_ctarank();
@@ -518,55 +518,71 @@ __global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBala
     __syncthreads();
     ptx::grid_dependency_wait();
 
-    // the CTA's tokens
     const int* cu = detail::stage_sequences(p, s_cu);
     const uint32_t first_sequence = detail::first_sequence_behind(p, cu, first);
-    for (uint32_t s = first_sequence; s < p.sequences; ++s) {
+
+    // selections of the CTA's tokens
+    for (uint32_t i = first * p.top + thread; i < last * p.top; i += kBalanceClusterThreads) {
+        const uint32_t token = i / p.top;
+        if (p.mask != nullptr && p.mask[token] == 0) continue;
+        const long long id = p.ids_64 != 0 ? static_cast<const long long*>(p.ids)[i] : static_cast<const int*>(p.ids)[i];
+        if (id < 0 || id >= static_cast<long long>(p.experts)) continue;
+        const uint32_t s = detail::first_sequence_behind(p, cu, token);
+        uint32_t begin = 0, end = 0;
+        if (s < p.sequences) detail::sequence_range(p, cu, s, begin, end);
+        if (token >= begin && token < end) atomicAdd(&s_counts[s * p.experts + static_cast<uint32_t>(id)], 1);
+    }
+    // Their probabilities: a strip of tokens for each warp.  A strip may touch several sequences; the sums of (warp, sequence) go to slot
+    // warp + sequence, which no other pair has.
+    const uint32_t strip = ceil_div(tokens_of_cta, kBalanceClusterWarps);
+    const uint32_t from = min(first + warp * strip, last), to = min(from + strip, last);
+    const uint32_t from_sequence = from < to ? detail::first_sequence_behind(p, cu, from) : p.sequences;
+    for (uint32_t s = from_sequence; s < p.sequences; ++s) {
         uint32_t begin, end;
         detail::sequence_range(p, cu, s, begin, end);
-        if (begin >= last) break;
-        begin = max(begin, first), end = min(end, last);
+        if (begin >= to) break;
+        begin = max(begin, from), end = min(end, to);
         if (begin >= end) continue;
-        detail::count_selections(p, begin, end, thread, kBalanceClusterThreads, s_counts + s * p.experts);
         float sums[kPerLane];
 #pragma unroll
         for (uint32_t c = 0; c < kPerLane; ++c) sums[c] = 0.0f;
         int counted = 0;
-        Row::add(p, begin, end, warp, kBalanceClusterWarps, lane, p.grad != nullptr ? s_rows : nullptr, first, sums, counted);
+        Row::add(p, begin, end, 0, 1, lane, p.grad != nullptr ? s_rows : nullptr, first, sums, counted);
         if (counted != 0) atomicAdd(&s_tokens[s], counted);
+        float* const into = s_slots + (warp + s - first_sequence) * p.experts;
 #pragma unroll
         for (uint32_t c = 0; c < kPerLane; ++c) {
 #pragma unroll
             for (uint32_t off = kLanes; off < 32; off *= 2) sums[c] += __shfl_xor_sync(0xffffffffu, sums[c], off);
             const uint32_t col = Row::column(lane, c);
-            if (lane < kLanes && col < p.experts) s_warps[warp * p.experts + col] = sums[c];
+            if (lane < kLanes && col < p.experts) into[col] = sums[c];
         }
-        __syncthreads();
-        for (uint32_t e = thread; e < p.experts; e += kBalanceClusterThreads) {
-            float sum = 0.0f;
-#pragma unroll
-            for (uint32_t w = 0; w < kBalanceClusterWarps; ++w) sum += s_warps[w * p.experts + e];
-            s_sums[s * p.experts + e] = sum;
-        }
-        __syncthreads();
     }
-    ptx::cluster_arrive(), ptx::cluster_wait();
-
-    // a of the sequences that the CTA's tokens belong to, and its share of the loss and the counts: every eighth pair
-    float loss = 0.0f;
-    for (uint32_t i = thread; i < at.pairs; i += kBalanceClusterThreads) {
+    __syncthreads();
+    for (uint32_t i = first_sequence * p.experts + thread; i < at.pairs; i += kBalanceClusterThreads) {
         const uint32_t s = i / p.experts;
         uint32_t begin, end;
         detail::sequence_range(p, cu, s, begin, end);
-        const bool share = i % kBalanceClusterCtas == rank, mine = begin < last && end > first;
-        if (!share && !mine) continue;
+        if (begin >= last) break;
+        begin = max(begin, first), end = min(end, last);
+        if (begin >= end) continue;
+        const uint32_t until = (end - 1 - first) / strip;
+        float sum = 0.0f;
+        for (uint32_t w = (begin - first) / strip; w <= until; ++w) sum += s_slots[(w + s - first_sequence) * p.experts + i % p.experts];
+        s_sums[i] = sum;
+    }
+    ptx::cluster_arrive(), ptx::cluster_wait();
+
+    // The CTA's share of the pairs: counts, the loss, and a, which every CTA of the cluster gets.
+    float loss = 0.0f;
+    const uint32_t share = ceil_div(at.pairs, kBalanceClusterCtas), until = min((rank + 1) * share, at.pairs);
+    for (uint32_t i = rank * share + thread; i < until; i += kBalanceClusterThreads) {
         const int count = detail::sum_of_cluster(s_counts + i);
-        const float weight = detail::balance_weight(p, count, detail::sum_of_cluster(s_tokens + s));
-        s_weights[i] = weight;
-        if (share) {
-            p.counts[i] = count;
-            loss = fmaf(weight, detail::sum_of_cluster(s_sums + i), loss);
-        }
+        const float weight = detail::balance_weight(p, count, detail::sum_of_cluster(s_tokens + i / p.experts));
+        p.counts[i] = count;
+        loss = fmaf(weight, detail::sum_of_cluster(s_sums + i), loss);
+#pragma unroll
+        for (uint32_t cta = 0; cta < kBalanceClusterCtas; ++cta) ptx::st_cluster_f32(ptx::map_to_cta(ptx::smem_u32(s_weights + i), cta), weight);
     }
 #pragma unroll
     for (uint32_t off = 16; off >= 1; off /= 2) loss += __shfl_xor_sync(0xffffffffu, loss, off);
@@ -578,32 +594,30 @@ __global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBala
         for (uint32_t w = 0; w < kBalanceClusterWarps; ++w) loss += s_loss[w];
         ptx::st_cluster_f32(ptx::map_to_cta(ptx::smem_u32(s_losses + rank), 0), loss);
     }
-    ptx::cluster_arrive();  // waited for at the end: nobody needs this CTA's memory any more, and the losses are there
-
-    if (p.grad != nullptr) {
-        float weights[kPerLane];
-        uint32_t done = first;  // tokens below have their gradient
-        for (uint32_t s = first_sequence; done < last; ++s) {
-            uint32_t begin = last, end = last;
-            if (s < p.sequences) detail::sequence_range(p, cu, s, begin, end);
-            begin = min(max(begin, done), last), end = min(max(end, begin), last);
-            if (begin < end) {
-#pragma unroll
-                for (uint32_t c = 0; c < kPerLane; ++c) {
-                    const uint32_t col = Row::column(lane, c);
-                    weights[c] = col < p.experts ? s_weights[s * p.experts + col] : 0.0f;
-                }
-            }
-            Row::grad(p, done, begin, end, warp, kBalanceClusterWarps, lane, s_rows, first, weights);
-            done = end;
-        }
-    }
-    ptx::cluster_wait();
+    ptx::cluster_arrive(), ptx::cluster_wait();  // behind it nobody looks at another CTA's memory
     if (rank == 0 && thread == 0) {
         loss = 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < kBalanceClusterCtas; ++i) loss += s_losses[i];
         *p.loss = loss;
+    }
+
+    if (p.grad == nullptr) return;
+    float weights[kPerLane];
+    uint32_t done = from;  // tokens below have their gradient
+    for (uint32_t s = from_sequence; done < to; ++s) {
+        uint32_t begin = to, end = to;
+        if (s < p.sequences) detail::sequence_range(p, cu, s, begin, end);
+        begin = min(max(begin, done), to), end = min(max(end, begin), to);
+        if (begin < end) {
+#pragma unroll
+            for (uint32_t c = 0; c < kPerLane; ++c) {
+                const uint32_t col = Row::column(lane, c);
+                weights[c] = col < p.experts ? s_weights[s * p.experts + col] : 0.0f;
+            }
+        }
+        Row::grad(p, done, begin, end, 0, 1, lane, s_rows, first, weights);
+        done = end;
     }
 }
 
@@ -705,9 +719,11 @@ inline int launch_balance(const BalanceParams& p, bool cluster, cudaStream_t str
         if (lanes <= 128) return launch_balance_as<T, kVec, 32, 4>(p, cluster, stream);
         return launch_balance_as<T, kVec, 32, 1024 / kVec / 32>(p, cluster, stream);
     }
-    // one expert per lane at a time: as few turns as the experts need
-    if (p.experts <= 32) return launch_balance_as<T, 1, 32, 1>(p, cluster, stream);
-    if (p.experts <= 64) return launch_balance_as<T, 1, 32, 2>(p, cluster, stream);
+    // one expert per lane at a time: rows of few experts share a warp
+    if (p.experts <= 8) return launch_balance_as<T, 1, 8, 1>(p, cluster, stream);
+    if (p.experts <= 16) return launch_balance_as<T, 1, 8, 2>(p, cluster, stream);
+    if (p.experts <= 32) return launch_balance_as<T, 1, 8, 4>(p, cluster, stream);
+    if (p.experts <= 64) return launch_balance_as<T, 1, 16, 4>(p, cluster, stream);
     if (p.experts <= 128) return launch_balance_as<T, 1, 32, 4>(p, cluster, stream);
     if (p.experts <= 256) return launch_balance_as<T, 1, 32, 8>(p, cluster, stream);
     if (p.experts <= 384) return launch_balance_as<T, 1, 32, 12>(p, cluster, stream);
