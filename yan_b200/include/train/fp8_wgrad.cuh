@@ -266,7 +266,8 @@ __device__ __forceinline__ void build_wgrad_schedule(const WgradParams& p, Wgrad
         if (g < p.groups.num_groups)
             s.origin = s.length[g] + p.whole_tiles % per_group * wgrad_length(p, s.blocks.block[g + 1] - s.blocks.block[g]);
         s.rest = at - s.origin;
-        s.stretches = max(min(gridDim.x / 2, s.rest / kWgradMinStretch), 1u);
+        // no more than pairs, or stretches of kWgradMinStretch, unless there are as many tiles; all of at least four k-blocks
+        s.stretches = max(min(gridDim.x / 2, max(s.rest / kWgradMinStretch, min(p.tiles - p.whole_tiles, s.rest / 4))), 1u);
         s.shortest = s.rest / s.stretches;
         s.longer = s.rest % s.stretches;
     }
@@ -413,11 +414,20 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
             __syncwarp();
             const uint32_t there = col < p.k && rows > rows16 * 16 ? rows - rows16 * 16 : 0u;  // rows
             if constexpr (kVector) {
+                auto read = [&](uint32_t i) {
+                    const uint32_t r = i * 4 + lane_row;
+                    return ptx::ld_shared_v4_f32(box + r * 128 + ((lane % 8 ^ (r & 7u)) << 4));
+                };
+                // bf16: all of them before the first is rounded and stored (zeros for 36 experts N=3446 K=2944: 285 -> 250 us; fp32
+                // gains nothing)
+                float4 values[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (sizeof(out_t) == 2) values[i] = read(i);
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i, to += step) {
-                    const uint32_t r = i * 4 + lane_row;
-                    float4 v = ptx::ld_shared_v4_f32(box + r * 128 + ((lane % 8 ^ (r & 7u)) << 4));
-                    if (r >= there) continue;
+                    float4 v = sizeof(out_t) == 2 ? values[i] : read(i);
+                    if (i * 4 + lane_row >= there) continue;
                     if constexpr (sizeof(out_t) == 4) {
                         if (accumulate) red_add4(to, v);
                         else *reinterpret_cast<float4*>(to) = v;
@@ -431,15 +441,22 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
                     }
                 }
             } else {
-#pragma unroll 4
+                float values[16];
+                [[maybe_unused]] float old_values[sizeof(out_t) == 2 ? 16 : 1];
+#pragma unroll
+                for (uint32_t r = 0; r < 16; ++r) {
+                    values[r] = ptx::ld_shared_f32(box + r * 128 + (((lane / 4) ^ (r & 7u)) << 4) + lane % 4 * 4);
+                    if constexpr (sizeof(out_t) == 2)
+                        old_values[r] = accumulate && r < there ? __bfloat162float(to[r * p.out_ld]) : 0.0f;
+                }
+#pragma unroll
                 for (uint32_t r = 0; r < 16; ++r, to += step) {
-                    const float v = ptx::ld_shared_f32(box + r * 128 + (((lane / 4) ^ (r & 7u)) << 4) + lane % 4 * 4);
                     if (r >= there) continue;
                     if constexpr (sizeof(out_t) == 4) {
-                        if (accumulate) red_add(to, v);
-                        else *to = v;
+                        if (accumulate) red_add(to, values[r]);
+                        else *to = values[r];
                     } else {
-                        *to = __float2bfloat16_rn(accumulate ? v + __bfloat162float(*to) : v);
+                        *to = __float2bfloat16_rn(values[r] + old_values[r]);
                     }
                 }
             }
