@@ -355,7 +355,7 @@ void yan_b200_adamw_step(const yan_b200_adamw_tensor* tensors, int num_tensors, 
  * id outside of [0, experts) is no selection.  token_mask: optional, a byte per token, 0 = does not count (its logits are not read).
  * cu_seqlens: optional int32 [sequences + 1] on the device, ascending; without it sequences = 1.  Tokens outside of every sequence do
  * not count; a sequence without tokens adds nothing.  loss: one fp32; counts int32 [sequences, experts]; grad: optional, of the
- * logits' type, zero for tokens that do not count.  experts <= 1024.
+ * logits' type, zero for tokens that do not count.  experts <= 1024; top and sequences <= 65535.
  * workspace: yan_b200_moe_balance_loss_workspace_bytes(...) bytes on a 256-byte boundary, 0 bytes (and a null pointer) for few tokens;
  * its content does not matter.
  */

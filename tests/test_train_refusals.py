@@ -54,7 +54,7 @@ def _adamw(numel=256, count=1, param=P, grad=P, m=P, v=P, ms=P, vs=P, copy=0, pa
                step, None, None)
 
 
-@pytest.mark.parametrize("change", [dict(numel=-1), dict(count=-1), dict(param=0), dict(grad=0), dict(m=0), dict(v=0), dict(param=P + 2),
+@pytest.mark.parametrize("change", [dict(numel=-1), dict(numel=1 << 62), dict(numel=1 << 62, bits=8), dict(count=-1), dict(param=0), dict(grad=0), dict(m=0), dict(v=0), dict(param=P + 2),
                                     dict(grad=P + 2), dict(m=P + 2), dict(v=P + 1), dict(copy=P + 1), dict(param_dtype=2), dict(grad_dtype=-1),
                                     dict(bits=16), dict(lr=-1.0), dict(lr=float("nan")), dict(lr=float("inf")), dict(beta1=1.0),
                                     dict(beta2=-0.1), dict(beta2=float("nan")), dict(eps=-1e-8), dict(step=0), dict(table=False),
@@ -74,7 +74,7 @@ def _balance(logits=P, ids=P, mask=None, cu=None, loss=P, counts=P, grad=P, t=20
                ws_bytes, None, sms)
 
 
-@pytest.mark.parametrize("change", [dict(t=-1), dict(e=0), dict(e=1025, ld=2048, grad_ld=2048), dict(top=0), dict(s=0), dict(s=2), dict(s=70000, cu=P),
+@pytest.mark.parametrize("change", [dict(t=-1), dict(e=0), dict(e=1025, ld=2048, grad_ld=2048), dict(top=0), dict(top=65536), dict(s=0), dict(s=2), dict(s=70000, cu=P),
                                     dict(ld=31), dict(grad_ld=31), dict(dtype=2), dict(score=2), dict(logits=None), dict(ids=None),
                                     dict(loss=None), dict(counts=None), dict(logits=P + 2), dict(grad=P + 1), dict(ids=P + 4), dict(ws=None),
                                     dict(ws=P + 16), dict(sms=0)])

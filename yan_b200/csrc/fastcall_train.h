@@ -248,7 +248,7 @@ PyObject* balance(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         const int64_t t = logits->size(0), e = logits->size(1), top = ids->size(1);
         int dtype;
         int64_t ld;
-        if (t > INT32_MAX || e < 1 || e > 1024 || ids->size(0) != t || !fits_int(top) || !element_type(*logits, &dtype) || !row_stride(*logits, &ld))
+        if (t > INT32_MAX || e < 1 || e > 1024 || ids->size(0) != t || top < 1 || top > 65535 || !element_type(*logits, &dtype) || !row_stride(*logits, &ld))
             return code(kNotTaken);
         const bool wide = ids->scalar_type() == at::kLong;
         if ((!wide && ids->scalar_type() != at::kInt) || !ids->is_contiguous()) return code(kNotTaken);

@@ -49,7 +49,7 @@ bool adamw_vector(const yan_b200_adamw_tensor& t, bool param_bf16, bool grad_bf1
 }
 
 bool adamw_tensor_ok(const yan_b200_adamw_tensor& t, bool param_bf16, bool grad_bf16, bool eight_bit) {
-    if (t.numel < 0) return false;
+    if (t.numel < 0 || t.numel / yan::adamw_chunk(eight_bit) >= 0x7fffffff) return false;  // a grid reaches over a tensor
     if (t.numel == 0) return true;
     if (t.param == nullptr || t.grad == nullptr || t.exp_avg == nullptr || t.exp_avg_sq == nullptr) return false;
     if (eight_bit && (t.exp_avg_scale == nullptr || t.exp_avg_sq_scale == nullptr)) return false;
@@ -165,7 +165,8 @@ YAN_EXPORT void yan_b200_moe_balance_loss(const void* logits, const void* expert
                                           float* loss, int* counts, void* grad, int tokens, int experts, int top, int sequences,
                                           long long logits_ld, long long grad_ld, int logits_dtype, int ids_64, int score, float coef,
                                           void* workspace, size_t workspace_bytes, void* stream, int num_sms, int* return_code) {
-    if (tokens < 0 || experts <= 0 || experts > static_cast<int>(yan::kMaxBalanceExperts) || top <= 0 || sequences <= 0 ||
+    if (tokens < 0 || experts <= 0 || experts > static_cast<int>(yan::kMaxBalanceExperts) || top <= 0 ||
+        top > static_cast<int>(yan::kMaxBalanceTop) || sequences <= 0 ||
         sequences > 65535 || num_sms <= 0 || loss == nullptr || counts == nullptr)
         return set_rc(return_code, yan::kBadArgument);
     if ((logits_dtype != YAN_B200_F32 && logits_dtype != YAN_B200_BF16) || (score != YAN_B200_SOFTMAX && score != YAN_B200_SIGMOID))

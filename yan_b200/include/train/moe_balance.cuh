@@ -20,6 +20,7 @@
 namespace yan {
 
 constexpr uint32_t kMaxBalanceExperts = 1024;
+constexpr uint32_t kMaxBalanceTop = 65535;  // the cluster kernel, for few tokens, counts selections in 32 bits
 constexpr uint32_t kBalanceThreads = 256, kBalanceWarps = kBalanceThreads / 32;
 
 struct BalanceParams {
@@ -88,7 +89,7 @@ __device__ __forceinline__ uint32_t first_sequence_behind(const BalanceParams& p
 template <typename T, uint32_t kVec, uint32_t kLanes, uint32_t kIter>
 struct BalanceRow {
     static constexpr uint32_t kPerLane = kVec * kIter, kGroups = 32 / kLanes;
-        static constexpr uint32_t kRows = kPerLane <= 2 ? 4 : kPerLane <= 8 ? 2 : 1, kRowsPerWarp = kGroups * kRows;
+    static constexpr uint32_t kRows = kPerLane <= 2 ? 4 : kPerLane <= 8 ? 2 : 1, kRowsPerWarp = kGroups * kRows;
 
     __device__ __forceinline__ static uint32_t column(uint32_t lane, uint32_t c) {
         return (c / kVec * kLanes + lane % kLanes) * kVec + c % kVec;
@@ -448,8 +449,10 @@ __global__ void __launch_bounds__(kBalanceThreads, kVec * kIter <= 16 ? 3 : 1) b
 }
 
 // ---- few tokens: one cluster ----
-// us for one cluster / for three launches: 64 x 64 6.1 / 8.2, 512 x 64 6.5 / 8.2, 512 x 256 9.4 / 9.5, 2048 x 64 10.0 / 8.7.
-constexpr uint32_t kBalanceClusterMaxLogits = 1u << 16;
+// A cluster has 128 warps: it wins while each has few tokens and few experts per lane.  us for one cluster / for three launches, one behind
+// the other in a graph, fp32: 64 x 64 4.9 / 6.5, 512 x 64 5.3 / 6.6, 128 x 512 7.6 / 11.8, 256 x 256 6.8 / 9.0, 1024 x 64 in 4 sequences
+// 8.1 / 8.0, 512 x 256 8.8 / 8.9, 1024 x 256 14.6 / 9.2, 2048 x 64 10.5 / 7.2, 4096 x 32 10.6 / 7.0, 8192 x 8 15.9 / 8.1.
+constexpr uint32_t kBalanceClusterMaxTokens = 1024, kBalanceClusterMaxLogits = 1u << 16;
 constexpr uint32_t kBalanceClusterCtas = 8, kBalanceClusterThreads = 512, kBalanceClusterWarps = kBalanceClusterThreads / 32;
 
 // Shared memory of a CTA, in words: per (sequence, expert) the sum, the selections and a; the slots of (warp, sequence) sums; per sequence its
@@ -536,7 +539,8 @@ __global__ void __launch_bounds__(kBalanceClusterThreads) __cluster_dims__(kBala
     // warp + sequence, which no other pair has.
     const uint32_t strip = ceil_div(tokens_of_cta, kBalanceClusterWarps);
     const uint32_t from = min(first + warp * strip, last), to = min(from + strip, last);
-    const uint32_t from_sequence = from < to ? detail::first_sequence_behind(p, cu, from) : p.sequences;
+    // not in front of the CTA's first, even where the ends of the sequences are out of order: the slots begin there
+    const uint32_t from_sequence = from < to ? max(detail::first_sequence_behind(p, cu, from), first_sequence) : p.sequences;
     for (uint32_t s = from_sequence; s < p.sequences; ++s) {
         uint32_t begin, end;
         detail::sequence_range(p, cu, s, begin, end);
@@ -632,7 +636,8 @@ struct BalanceWorkspace {
 
 inline BalanceWorkspace plan_balance_workspace(uint32_t tokens, uint32_t experts, uint32_t sequences, bool with_grad, uint32_t num_sms) {
     BalanceWorkspace w = {};
-    w.cluster = num_sms >= kBalanceClusterCtas && static_cast<uint64_t>(tokens) * experts <= kBalanceClusterMaxLogits;
+    w.cluster = num_sms >= kBalanceClusterCtas && tokens <= kBalanceClusterMaxTokens &&
+                static_cast<uint64_t>(tokens) * experts <= kBalanceClusterMaxLogits;
     if (w.cluster) {
         w.strip_tokens = ceil_div(tokens, kBalanceClusterCtas);
         w.cluster = static_cast<uint64_t>(experts) * sequences <= 16384 &&

@@ -11,6 +11,7 @@ from . import utils as _utils
 from .utils import get_num_sms
 
 MAX_EXPERTS = 1024
+MAX_TOP = 65535
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _SCORES = {"softmax": 0, "sigmoid": 1}
 
@@ -33,9 +34,9 @@ def moe_balance_loss(logits: torch.Tensor, expert_ids: torch.Tensor, *, coef: fl
     what the rest of the model sends back; None with with_grad=False.  counts, int32 [S, E], are the group sizes of
     k_grouped_fp8_linear_wgrad and masked_m of m_grouped_gemm_fp8_fp8_bf16_nt_masked (for S = 1).
 
-    logits [T, E] fp32 or bf16, E <= 1024, rows may be strided; expert_ids [T, top] int64 or int32, contiguous, an id outside of
+    logits [T, E] fp32 or bf16, E <= 1024, rows may be strided; expert_ids [T, top <= 65535] int64 or int32, contiguous, an id outside of
     [0, E) selects nothing (a dropped token).  token_mask [T] bool: tokens that count; the logits of the others are not read and their
-    gradient is zero.  cu_seqlens int32 [S + 1], ascending, on the device: sequence s is tokens [cu_seqlens[s], cu_seqlens[s + 1]); without it
+    gradient is zero.  cu_seqlens int32 [S + 1], S <= 65535, ascending, on the device: sequence s is tokens [cu_seqlens[s], cu_seqlens[s + 1]); without it
     all tokens are one sequence.  A sequence without tokens adds nothing.  loss is an fp32 tensor without dimensions."""
     if with_grad and grad is None and workspace is None and _utils._num_sms is not None and score in _SCORES:
         result = _lib.fast().balance(logits, expert_ids, token_mask, cu_seqlens, coef, _SCORES[score], _utils._num_sms)
@@ -47,7 +48,7 @@ def moe_balance_loss(logits: torch.Tensor, expert_ids: torch.Tensor, *, coef: fl
     assert logits.dim() == 2 and logits.dtype in _DTYPES, "logits are [T, E] in fp32 or bf16"
     t, e = logits.shape
     assert 0 < e <= MAX_EXPERTS and (e == 1 or logits.stride(1) == 1)
-    assert expert_ids.device == logits.device and expert_ids.dim() == 2 and expert_ids.shape[0] == t and expert_ids.shape[1] > 0
+    assert expert_ids.device == logits.device and expert_ids.dim() == 2 and expert_ids.shape[0] == t and 0 < expert_ids.shape[1] <= MAX_TOP
     assert expert_ids.dtype in (torch.int64, torch.int32) and expert_ids.is_contiguous()
     assert score in _SCORES, "score is 'softmax' or 'sigmoid'"
     if token_mask is not None:
@@ -56,7 +57,7 @@ def moe_balance_loss(logits: torch.Tensor, expert_ids: torch.Tensor, *, coef: fl
     if cu_seqlens is not None:
         assert cu_seqlens.device == logits.device and cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous()
         sequences = cu_seqlens.numel() - 1
-        assert sequences > 0
+        assert 0 < sequences <= 65535
     if grad is not None:
         assert with_grad and grad.device == logits.device and grad.dtype == logits.dtype and grad.shape == (t, e)
         assert e == 1 or grad.stride(1) == 1
