@@ -300,7 +300,8 @@ enum { YAN_B200_F32 = 0, YAN_B200_BF16 = 1 };
  * 16 columns are the fast case); out [n, out_ld] fp32 or bf16, rounded once.  accumulate != 0: added to what out holds.  m = 0 is a sum
  * of nothing.  What is not finite in a column of dy (x) makes that row (column) of out NaN.
  * workspace: yan_b200_fp8_linear_wgrad_workspace_bytes(m, n, k, 0, num_sms) bytes on a 256-byte boundary for the codes, scales and
- * partial tiles; its content does not matter.  Calls that may overlap need one each.
+ * partial tiles; its content does not matter.  Calls that may overlap need one each.  m <= 65535 * 128 (with groups m / 128 + num_groups
+ * <= 65535).  The products run on num_sms / 2 pairs of SMs, one at least.
  */
 size_t yan_b200_fp8_linear_wgrad_workspace_bytes(int m, int n, int k, int num_groups, int num_sms);
 void yan_b200_fp8_linear_wgrad(const void* dy, const void* x, void* out, int m, int n, int k, long long dy_ld, long long x_ld,

@@ -2,7 +2,8 @@
 
 Public names follow the reference's package (yan/__init__.py:1-5): `jit`, `gemm` (the operator
 module, which here also holds the callables the reference never wrote), `bench_kineto`, `calc_diff`,
-`get_col_major_tensor`.  The kernels are CUDA only; importing an operator without the built library
+`get_col_major_tensor`.  Beside them: the operators that train such layers (`fp8_linear_wgrad`,
+`k_grouped_fp8_linear_wgrad`, `adamw_step`, `moe_balance_loss`).  The kernels are CUDA only; importing an operator without the built library
 raises (no CPU or PyTorch fallback exists).
 """
 from . import jit

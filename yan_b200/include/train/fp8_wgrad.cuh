@@ -191,9 +191,9 @@ struct WgradSchedule {
 
 // A pair of CTAs computes 256 x kCols of dW at a time, each CTA 128 rows of it: per 128 tokens it loads 128 rows of A and kCols / 2 columns of
 // B, where a CTA by itself would load all kCols.  What bounds long sums is the power limit (1.28 GHz at N=28672 K=8192), so that bytes
-// moved per product count more than cycles: quantization and products together there 1.74 ms with pairs and 256 columns, 1.81 with 192
-// (whose two accumulators lie side by side, so that nothing ever waits for sums to be read), 2.12 with 224, 1.95 with single CTAs of
-// 128 x 256.
+// moved per product count more than cycles.  Quantization and products together take 1.66 ms there; when the tiles were chosen it was 1.74
+// with pairs and 256 columns, 1.81 with 192 (whose two accumulators lie side by side, so that nothing ever waits for sums to be read),
+// 2.12 with 224, 1.95 with single CTAs of 128 x 256.
 constexpr uint32_t kWgradRows = 256;
 // Parts of a tile that meet in L2 cost about as much as twelve k-blocks (us with the shortest tile that is cut and the shortest stretch at
 // 8 and 8, 24 and 12, 32 and 16 k-blocks: 2048 tokens N=1024 K=512 18.5, 14.8, 14.8; 3888 tokens N=K=128 16.8, 16.1, 14.9; 4096
@@ -205,7 +205,8 @@ struct WgradTile {
     static constexpr uint32_t kStages = 6;
     // k-blocks that are summed in tensor memory before the sums move to registers.  An addition there rounds towards zero: 8192 tokens of
     // uneven size, relative error 1.3e-6 in one chain of 64 k-blocks, 5e-7 in chains of 32, 2.2e-7 in chains of 16.  Where the
-    // accumulators share columns the products wait at the end of a chain: N=28672 K=8192, 8192 tokens, 1.72, 1.74 and 1.85 ms.
+    // accumulators share columns the products wait at the end of a chain: N=28672 K=8192, 8192 tokens, 1.72, 1.74 and 1.85 ms
+    // (1.66 with 32 now).
     static constexpr uint32_t kChain = kCols <= 192 ? 16 : 32;
     static constexpr uint32_t kStageA = kMnBoxBytes, kStageB = kMnBoxBytes;
     static constexpr uint32_t kScaleTiles = 1 + ceil_div(kCols, 128u);
