@@ -200,9 +200,14 @@ constexpr uint32_t kWgradRows = 256;
 // tokens N=K=4000 83.6, 84.2, 78.7).
 constexpr uint32_t kWgradMinCut = 32, kWgradMinStretch = 16, kWgradMaxStoreCost = 20;
 
-template <uint32_t kCols>
+// kOldItem: bytes of an element of dW whose old values are fetched ahead of the store that adds to them, or 0.  They wait in shared memory, and what
+// counts is how many bytes are on their way; stages of products make room (us for fp32 in 16 experts N=4096 K=2048, 16384 tokens: added in L2
+// 350; two boxes of a warp fetched ahead at five stages 345, four at four 300, six at three 287 but slower elsewhere; 8192 tokens
+// N=7168 K=2048, where products count: 131, 131, 138, 156.  bf16, old values in registers a box ahead at six stages, four boxes at five
+// and six at four: 326, 273 and 290; 126, 128 and 138).
+template <uint32_t kCols, uint32_t kOldItem>
 struct WgradTile {
-    static constexpr uint32_t kStages = 6;
+    static constexpr uint32_t kStages = kOldItem == 0 ? 6 : kOldItem == 2 ? 5 : 4;
     // k-blocks that are summed in tensor memory before the sums move to registers.  An addition there rounds towards zero: 8192 tokens of
     // uneven size, relative error 1.3e-6 in one chain of 64 k-blocks, 5e-7 in chains of 32, 2.2e-7 in chains of 16.  Where the
     // accumulators share columns the products wait at the end of a chain: N=28672 K=8192, 8192 tokens, 1.72, 1.74 and 1.85 ms
@@ -214,7 +219,9 @@ struct WgradTile {
     static constexpr uint32_t kOffA = 0, kOffB = kOffA + kStages * kStageA, kOffScales = kOffB + kStages * kStageB;
     static constexpr uint32_t kBoxBytes = 16 * 128;  // output staging, one box per warp
     static constexpr uint32_t kOffStore = kOffScales + kStages * kStageScales;
-    static constexpr uint32_t kOffSchedule = kOffStore + 8 * kBoxBytes;
+    static constexpr uint32_t kOldBoxes = kOldItem == 0 ? 0 : 4, kOldBoxBytes = 16 * 32 * kOldItem;
+    static constexpr uint32_t kOffOld = kOffStore + 8 * kBoxBytes;
+    static constexpr uint32_t kOffSchedule = kOffOld + 8 * kOldBoxes * kOldBoxBytes;
     static constexpr uint32_t kOffBarriers = align_up(kOffSchedule + static_cast<uint32_t>(sizeof(WgradSchedule)), 8u);
     static constexpr uint32_t kNumBarriers = 2 * kStages + 6;
     static constexpr uint32_t kOffTmemSlot = kOffBarriers + kNumBarriers * 8, kOffAbort = kOffTmemSlot + 4;
@@ -227,6 +234,7 @@ struct WgradTile {
     static constexpr uint32_t kTmemSecond = kCols - kShared, kTmemScales = kTmemSecond + kCols;
     static_assert(kCols % 32 == 0 && kTmemScales + 3 * kTmemScaleSet <= kTmemCols && kShared <= kWarpCols);
     static_assert(kSmemSize <= 232448);
+    static_assert(kStages <= 6 && kOldBoxes <= kWarpCols / 16);
     static_assert(kChain % 4 == 0 && kWgradMinCut % 4 == 0 && kWgradMinStretch >= 8);
 };
 
@@ -363,17 +371,65 @@ __device__ __forceinline__ void red_add4(float* p, const float4& v) {
     asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
+// The old values of dW on their way to a warp that adds them (fp32, vectors): boxes of 16 rows x 32 columns in the order in which they
+// are stored are fetched into shared memory several boxes ahead, across the end of a tile, each lane the vectors that it adds itself.
+template <typename out_t>
+struct WgradOldRows {
+    const out_t* from;  // this lane's vector in the first of its rows, which are four apart, and the leftmost 32 columns
+    uint32_t rows;      // rows of the tile that dW has; zero where nothing is fetched
+    uint32_t col;
+
+    // Only what no other pair adds to, and if there is something to add.
+    __device__ __forceinline__ static bool fetched(const WgradUnit& u) { return u.first_pair == u.last_pair && u.blocks != 0; }
+    __device__ __forceinline__ WgradOldRows(const WgradParams& p, const WgradUnit& u, bool exists, uint32_t row_in_tile, uint32_t leftmost,
+                                            uint32_t lane) {
+        const uint32_t row0 = u.row0 + row_in_tile;
+        rows = exists && fetched(u) && row0 < p.n ? min(p.n - row0, 32u) : 0u;
+        col = u.col0 + leftmost + lane % 8 * 4;
+        from = static_cast<const out_t*>(p.out) + u.group * p.out_group + static_cast<uint64_t>(row0 + lane / 8) * p.out_ld + col;
+    }
+    // One group of copies, whether there is something to fetch or not.
+    __device__ __forceinline__ void fetch(const WgradParams& p, uint32_t number, uint32_t direction, uint32_t box, uint32_t lane) const {
+        const uint32_t rows16 = number % 2;
+        const int right = static_cast<int>(32 * direction * (number / 2));
+        if (col + right < p.k) {
+#pragma unroll
+            for (uint32_t i = rows16 * 4; i < rows16 * 4 + 4; ++i)
+                if (i * 4 + lane / 8 < rows) {
+                    const out_t* src = from + i * 4 * p.out_ld + right;
+                    if constexpr (sizeof(out_t) == 4) ptx::cp_async_16(box + (i % 4 * 32 + lane) * 16, src);
+                    else ptx::cp_async_8(box + (i % 4 * 32 + lane) * 8, src);
+                }
+        }
+        ptx::cp_async_commit();
+    }
+};
+
+// The boxes of a warp in turn.
+template <uint32_t kBoxes, uint32_t kBytes>
+struct WgradOldRing {
+    uint32_t first, now;
+    __device__ __forceinline__ void advance() { now = now + kBytes == first + kBoxes * kBytes ? first : now + kBytes; }
+    template <typename out_t>
+    __device__ __forceinline__ void fill(const WgradParams& p, const WgradOldRows<out_t>& rows, uint32_t direction, uint32_t lane) {
+#pragma unroll
+        for (uint32_t i = 0; i < kBoxes; ++i, advance()) rows.fetch(p, i, direction, now, lane);
+    }
+};
+
 // Stores a warp's 32 rows x kWarpCols columns; lane r holds row r, acc[c] column first_col + c / 16 * 16 * direction + c % 16.  They go
 // through the warp's box in shared memory, 16 rows x 32 columns in fp32 at a time, so that a store instruction covers four pieces of 128
 // contiguous bytes (kVector; otherwise one, an element per lane).  16-byte chunk j of box row r is at chunk j ^ r % 8.
 // What bounds it is the number of pieces: an SM sends one in two cycles, whatever its size (pieces of 64 bytes: 6400 cycles for the 128 x 256
 // of a CTA).
-// fp32 is added to what dW holds where dW lies, in L2: every element once, so that the order does not matter, and nothing waits for the
-// old value (16 experts N=4096 K=2048, 16384 tokens: loads and stores at the end of a tile took twice as long, loads of the next
-// tile's old values ahead of its products 1.5 times).  bf16 is loaded, added in 32 bits and rounded once.
-template <typename out_t, uint32_t kWarpCols, bool kVector>
+// What dW holds is fetched ahead (kOldBoxes), or fp32 is added to it where it lies, in L2: every element once, so that the order does not
+// matter, and nothing waits for the old value.  The sum is the same.  (16 experts N=4096 K=2048, 16384 tokens: loads and stores at the end
+// of a tile took twice as long as adding in L2, old values in registers a pass ahead 1.1 times: few of them are on their way at a time.)
+// bf16 is added in 32 bits and rounded once.
+template <typename out_t, uint32_t kWarpCols, bool kVector, uint32_t kOldBoxes = 0, typename Ring = int>
 __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const WgradUnit& u, uint32_t box, uint32_t row_in_tile, uint32_t first_col,
-                                                 uint32_t direction, uint32_t lane, const float (&acc)[kWarpCols]) {
+                                                 uint32_t direction, uint32_t lane, const float (&acc)[kWarpCols],
+                                                 [[maybe_unused]] Ring* ring = nullptr, [[maybe_unused]] const WgradOldRows<out_t>* after = nullptr) {
     static_assert(kWarpCols % 32 == 0);
     const uint32_t row0 = u.row0 + row_in_tile;
     if (row0 >= p.n) return;
@@ -387,20 +443,10 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
     out_t* dst = reinterpret_cast<out_t*>(p.out) + u.group * p.out_group + static_cast<uint64_t>(row0 + lane_row) * p.out_ld + col;
     const uint64_t step = kRowStep * p.out_ld;
     const bool accumulate = p.accumulate != 0;
-    // bf16, vectors: the old values of a pass are fetched one pass ahead
-    constexpr bool kFetch = sizeof(out_t) == 2 && kVector;
-    [[maybe_unused]] uint2 old[kFetch ? 8 : 1], next_old[kFetch ? 8 : 1];
-    auto fetch = [&](uint2 (&into)[kFetch ? 8 : 1], const out_t* from, uint32_t at_col) {
-#pragma unroll
-        for (uint32_t i = 0; i < (kFetch ? 8 : 0); ++i)
-            if (at_col < p.k && i * 4 + lane_row < rows) into[i] = *reinterpret_cast<const uint2*>(from + i * step);
-    };
-    if (kFetch && accumulate) fetch(old, dst, col);
+    [[maybe_unused]] const WgradOldRows<out_t> here(p, u, kOldBoxes != 0, row_in_tile, direction == 1 ? first_col : first_col - 16, lane);
 #pragma unroll
     for (uint32_t pass = 0; pass < kWarpCols / 32; ++pass) {
         out_t* to = dst;
-        if (kFetch && accumulate && pass + 1 < kWarpCols / 32)
-            fetch(next_old, dst + static_cast<int>(32 * direction), col + 32 * direction);
 #pragma unroll
         for (uint32_t rows16 = 0; rows16 < 2; ++rows16) {
             __syncwarp();  // the read-back in front is over
@@ -414,6 +460,29 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
             }
             __syncwarp();
             const uint32_t there = col < p.k && rows > rows16 * 16 ? rows - rows16 * 16 : 0u;  // rows
+            if constexpr (kOldBoxes != 0) {
+                ptx::cp_async_wait_group<kOldBoxes - 1>();
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i, to += step) {
+                    const uint32_t r = i * 4 + lane_row;
+                    [[maybe_unused]] float4 v = ptx::ld_shared_v4_f32(box + r * 128 + ((lane % 8 ^ (r & 7u)) << 4));
+                    if constexpr (sizeof(out_t) == 4) {
+                        const float4 o = ptx::ld_shared_v4_f32(ring->now + (i * 32 + lane) * 16);
+                        if (r < there) *reinterpret_cast<float4*>(to) = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+                    } else {
+                        const uint2 o = ptx::ld_shared_v2(ring->now + (i * 32 + lane) * 8);
+                        v.x += __uint_as_float(o.x << 16), v.y += __uint_as_float(o.x & 0xFFFF0000u);
+                        v.z += __uint_as_float(o.y << 16), v.w += __uint_as_float(o.y & 0xFFFF0000u);
+                        if (r < there) *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+                    }
+                }
+                __syncwarp();
+                const uint32_t number = pass * 2 + rows16 + kOldBoxes;
+                if (number < kWarpCols / 16) here.fetch(p, number, direction, ring->now, lane);
+                else after->fetch(p, number - kWarpCols / 16, direction, ring->now, lane);
+                ring->advance();
+                continue;
+            }
             if constexpr (kVector) {
                 auto read = [&](uint32_t i) {
                     const uint32_t r = i * 4 + lane_row;
@@ -422,9 +491,14 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
                 // bf16: all of them before the first is rounded and stored (zeros for 36 experts N=3446 K=2944: 285 -> 250 us; fp32
                 // gains nothing)
                 float4 values[4];
+                [[maybe_unused]] uint2 old_values[4];  // of a tile that others had a part in, too: not fetched ahead
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i)
-                    if (sizeof(out_t) == 2) values[i] = read(i);
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if constexpr (sizeof(out_t) == 2) {
+                        values[i] = read(i);
+                        if (accumulate && i * 4 + lane_row < there) old_values[i] = *reinterpret_cast<const uint2*>(to + i * step);
+                    }
+                }
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i, to += step) {
                     float4 v = sizeof(out_t) == 2 ? values[i] : read(i);
@@ -434,7 +508,7 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
                         else *reinterpret_cast<float4*>(to) = v;
                     } else {
                         if (accumulate) {
-                            const uint2 o = old[rows16 * 4 + i];
+                            const uint2 o = old_values[i];
                             v.x += __uint_as_float(o.x << 16), v.y += __uint_as_float(o.x & 0xFFFF0000u);
                             v.z += __uint_as_float(o.y << 16), v.w += __uint_as_float(o.y & 0xFFFF0000u);
                         }
@@ -462,10 +536,6 @@ __device__ __forceinline__ void store_wgrad_rows(const WgradParams& p, const Wgr
                 }
             }
         }
-        if constexpr (kFetch) {
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) old[i] = next_old[i];
-        }
         col += 32 * direction;
         dst += static_cast<int>(32 * direction);
     }
@@ -478,11 +548,11 @@ struct WgradMaps {
     CUtensorMap scales_n, scales_k;  // their scale tiles: a box is what a tile of products needs
 };
 
-template <uint32_t kCols, typename out_t, bool kVector>
+template <uint32_t kCols, typename out_t, bool kVector, bool kOldAhead>
 __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
     fp8_wgrad_kernel(const WgradParams p, const __grid_constant__ WgradMaps maps) {
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ >= 1000)
-    using T = WgradTile<kCols>;
+    using T = WgradTile<kCols, kOldAhead ? sizeof(out_t) : 0>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
     WgradSchedule& schedule = *reinterpret_cast<WgradSchedule*>(smem + T::kOffSchedule);
@@ -643,9 +713,17 @@ __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
         const uint32_t box = ptx::smem_u32(smem + T::kOffStore + part * T::kBoxBytes);
         const uint32_t empty_of_pair = ptx::map_to_cta(ptx::smem_u32(sums_empty), 0);
         [[maybe_unused]] const uint32_t shared_of_pair = ptx::map_to_cta(ptx::smem_u32(shared_empty), 0);
+        const uint32_t row_in_tile = rank * 128 + quarter * 32;
+        [[maybe_unused]] const uint32_t leftmost = direction == 1 ? first_col : first_col - 16;
+        const uint32_t old_boxes = ptx::smem_u32(smem + T::kOffOld) + part * T::kOldBoxes * T::kOldBoxBytes;
+        [[maybe_unused]] detail::WgradOldRing<T::kOldBoxes, T::kOldBoxBytes> ring{old_boxes, old_boxes};
+        [[maybe_unused]] detail::WgradUnit after;  // the unit behind this one
         uint32_t buf = 0, sums_phase = 0;
-        bool alive = true;
-        while (alive && walk.next(p, schedule, u)) {
+        bool alive = true, more = walk.next(p, schedule, u);
+        if constexpr (kOldAhead) {
+            ring.fill(p, detail::WgradOldRows<out_t>(p, u, more, row_in_tile, leftmost, lane), direction, lane);
+        }
+        while (alive && more) {
             float acc[kWarpCols];
 #pragma unroll
             for (uint32_t j = 0; j < kWarpCols; ++j) acc[j] = 0.0f;
@@ -676,6 +754,7 @@ __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
                 if (buf == 0) sums_phase ^= 1;
             }
             if (!alive || *abort_flag != 0) break;  // a wait ran out: the sums may be incomplete
+            bool complete = true;  // here are all sums of the tile
             if (u.first_pair != u.last_pair) {
                 // Partial tiles meet in L2; who counts itself last adds them in the order of the tokens.  A pair begins at most one tile
                 // that others end, and ends at most one that another began: a slot for each.
@@ -690,24 +769,41 @@ __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
                 __syncwarp();
                 uint32_t before = 0;
                 if (lane == 0) before = atomicAdd(p.counters + (u.first_pair * 2 + rank) * 8 + part, 1u);
-                if (__shfl_sync(0xffffffffu, before, 0) != u.last_pair - u.first_pair) continue;
-                __threadfence();
+                complete = __shfl_sync(0xffffffffu, before, 0) == u.last_pair - u.first_pair;
+                if (complete) {
+                    __threadfence();
 #pragma unroll
-                for (uint32_t j = 0; j < kWarpCols; ++j) acc[j] = 0.0f;
+                    for (uint32_t j = 0; j < kWarpCols; ++j) acc[j] = 0.0f;
 #pragma unroll 1
-                for (uint32_t pair = u.first_pair; pair <= u.last_pair; ++pair) {
-                    const float4* from = slot(pair);
+                    for (uint32_t pair = u.first_pair; pair <= u.last_pair; ++pair) {
+                        const float4* from = slot(pair);
 #pragma unroll
-                    for (uint32_t j = 0; j < kWarpCols / 4; ++j) {
-                        const float4 f = __ldcg(from + j * 32);
-                        acc[4 * j] += f.x, acc[4 * j + 1] += f.y, acc[4 * j + 2] += f.z, acc[4 * j + 3] += f.w;
+                        for (uint32_t j = 0; j < kWarpCols / 4; ++j) {
+                            const float4 f = __ldcg(from + j * 32);
+                            acc[4 * j] += f.x, acc[4 * j + 1] += f.y, acc[4 * j + 2] += f.z, acc[4 * j + 3] += f.w;
+                        }
                     }
                 }
-            } else if (u.blocks == 0 && p.accumulate != 0) {
-                continue;
             }
-            detail::store_wgrad_rows<out_t, kWarpCols, kVector>(p, u, box, rank * 128 + quarter * 32, first_col, direction, lane, acc);
+            if constexpr (kOldAhead) {
+                more = walk.next(p, schedule, after);
+                const detail::WgradOldRows<out_t> rows(p, after, more, row_in_tile, leftmost, lane);
+                if (detail::WgradOldRows<out_t>::fetched(u) && u.row0 + row_in_tile < p.n) {
+                    detail::store_wgrad_rows<out_t, kWarpCols, kVector, T::kOldBoxes>(p, u, box, row_in_tile, first_col, direction, lane, acc,
+                                                                                      &ring, &rows);
+                } else {
+                    if (complete && u.blocks != 0)
+                        detail::store_wgrad_rows<out_t, kWarpCols, kVector>(p, u, box, row_in_tile, first_col, direction, lane, acc);
+                    ring.fill(p, rows, direction, lane);
+                }
+                u = after;
+            } else {
+                if (complete && (u.blocks != 0 || p.accumulate == 0))
+                    detail::store_wgrad_rows<out_t, kWarpCols, kVector>(p, u, box, row_in_tile, first_col, direction, lane, acc);
+                more = walk.next(p, schedule, u);
+            }
         }
+        if constexpr (kOldAhead) ptx::cp_async_wait_all();
         __syncwarp();
     }
     ptx::tcgen05_fence_before_thread_sync();
@@ -805,9 +901,9 @@ inline CUtensorMap make_scale_tiles_desc(const void* base, uint64_t tiles, uint3
     return map;
 }
 
-template <uint32_t kCols, typename out_t, bool kVector>
+template <uint32_t kCols, typename out_t, bool kVector, bool kOldAhead = false>
 inline int launch_wgrad_products(const WgradParams& p, const WgradMaps& maps, uint32_t pairs, cudaStream_t stream) {
-    constexpr uint32_t kSmem = WgradTile<kCols>::kSmemSize;
+    constexpr uint32_t kSmem = WgradTile<kCols, kOldAhead ? sizeof(out_t) : 0>::kSmemSize;
     int device = 0, max_smem = 0;
     if (cudaGetDevice(&device) != cudaSuccess) return kLaunchFailed;
     cudaDeviceGetAttribute(&max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
@@ -822,7 +918,7 @@ inline int launch_wgrad_products(const WgradParams& p, const WgradMaps& maps, ui
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    auto kernel = fp8_wgrad_kernel<kCols, out_t, kVector>;
+    auto kernel = fp8_wgrad_kernel<kCols, out_t, kVector, kOldAhead>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)) != cudaSuccess ||
         cudaLaunchKernelEx(&cfg, kernel, p, maps) != cudaSuccess) {
         cudaGetLastError();
@@ -905,9 +1001,18 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
     p.counters = reinterpret_cast<uint32_t*>(ws + w.counters);
     p.status = a.status;
     p.timeout_ns = a.timeout_ns;
+    // Old values are fetched ahead in bf16, and in fp32 where a tile has few k-blocks and its store is what takes long: us for 8, 16, 32 and 64
+    // k-blocks per group (16 experts N=4096 K=2048; one N=7168 K=2048; 8 N=K=4096; one N=7168 K=2048) added in L2 350, 51.5, 585, 131, fetched
+    // ahead 300, 50.1, 610, 138.  With a tile for each pair at most there is nothing to hide them behind (333 tokens N=1032 K=520 12.4, 12.8).
+    const bool ahead = a.accumulate && (a.out_bf16 || (w.tiles > w.pairs && a.groups.rows <= 16u * 128 * a.groups.num_groups));
     auto launch = [&](auto out, auto vectors) {
         using out_t = decltype(out);
         constexpr bool kVector = decltype(vectors)::value;
+        if constexpr (kVector) {
+            if (ahead)
+                return w.cols == 192 ? launch_wgrad_products<192, out_t, true, true>(p, maps, w.pairs, stream)
+                                     : launch_wgrad_products<256, out_t, true, true>(p, maps, w.pairs, stream);
+        }
         return w.cols == 192 ? launch_wgrad_products<192, out_t, kVector>(p, maps, w.pairs, stream)
                              : launch_wgrad_products<256, out_t, kVector>(p, maps, w.pairs, stream);
     };
