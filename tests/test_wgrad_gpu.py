@@ -226,3 +226,42 @@ def test_is_the_gradient(cuda_lib):
         # (tokens / 32 + 4) 2^-22 of the magnitudes in fp32, 2^-40 in the differences
         bound = (260 / 32 + 4) * 2.0 ** -22 * ((a.abs().t() @ b.abs()) * d.abs()).sum() + 2.0 ** -40 * (a.abs() * (b.abs() @ w.abs().t())).sum()
         assert (slope - (out * d).sum()).abs() <= bound
+
+
+@pytest.mark.parametrize("sms", [2, 6, 14])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(300, 700, 392), (300, 300, 188), (1, 1000, 768), (2048, 520, 960), (5000, 530, 380), (8200, 260, 572)])
+def test_accumulate_with_several_tiles_per_pair(cuda_lib, monkeypatch, sms, dtype, m, n, k):
+    """What the matrix holds is fetched while the tile in front is stored: tiles whose rows or columns end early, tiles that pairs share
+    between whole ones, both widths of tiles; a slice of a wider matrix, whose surroundings keep their values."""
+    import yan_b200
+    from yan_b200.jit_kernels import utils
+    monkeypatch.setattr(utils, "_num_sms", sms)
+    dy, x = _inputs(m, n, k, seed=sms)
+    wide = (torch.randn(n, k + 24, device="cuda") * 0.05).to(dtype)
+    before = wide.clone()
+    yan_b200.fp8_linear_wgrad(dy, x, out=wide[:, 8:8 + k], accumulate=True)
+    _check(wide[:, 8:8 + k], *train.weight_grad(dy, x), m, before[:, 8:8 + k])
+    assert torch.equal(wide[:, :8], before[:, :8]) and torch.equal(wide[:, 8 + k:], before[:, 8 + k:])
+    assert yan_b200.read_device_status() == 0
+
+
+@pytest.mark.parametrize("sms", [2, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sizes", [[0, 130, 1, 0, 700, 257], [64] * 20, [0, 0, 0], [4200, 0, 90]])
+def test_accumulate_over_groups_with_several_tiles_per_pair(cuda_lib, monkeypatch, sms, dtype, sizes):
+    import yan_b200
+    from yan_b200.jit_kernels import utils
+    monkeypatch.setattr(utils, "_num_sms", sms)
+    n, k = 300, 264
+    dy, x = _inputs(max(sum(sizes), 1), n, k, seed=sms)
+    lengths = torch.tensor(sizes, dtype=torch.int32, device="cuda")
+    starts = lengths.cumsum(0).to(torch.int32) - lengths
+    old = (torch.randn(len(sizes), n, k, device="cuda") * 0.05).to(dtype)
+    out = old.clone()
+    yan_b200.k_grouped_fp8_linear_wgrad(dy, x, starts, lengths, out=out, accumulate=True)
+    for g, (start, size) in enumerate(zip(starts.tolist(), sizes)):
+        if size == 0:
+            assert torch.equal(out[g], old[g])
+        else:
+            _check(out[g], *train.weight_grad(dy[start:start + size], x[start:start + size]), size, old[g])
