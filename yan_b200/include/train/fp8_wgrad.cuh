@@ -189,7 +189,7 @@ struct WgradSchedule {
     uint32_t stretches, shortest, longer;  // the first `longer` stretches are one longer than `shortest`
 };
 
-// A pair of CTAs computes 256 x kCols of dW at a time, each CTA 128 rows of it: per 128 tokens it loads 128 rows of A and kCols / 2 columns of
+// A pair of CTAs computes 256 x kCols of dW at a time (64, 128, 192 or 256: choose_wgrad_cols), each CTA 128 rows of it: per 128 tokens it loads 128 rows of A and kCols / 2 columns of
 // B, where a CTA by itself would load all kCols.  What bounds long sums is the power limit (1.28 GHz at N=28672 K=8192), so that bytes
 // moved per product count more than cycles.  Quantization and products together take 1.66 ms there; when the tiles were chosen it was 1.74
 // with pairs and 256 columns, 1.81 with 192 (whose two accumulators lie side by side, so that nothing ever waits for sums to be read),
@@ -848,8 +848,18 @@ inline uint32_t choose_whole_wgrad_tiles(uint32_t tiles, uint32_t pairs) {
     return (2 * rest > pairs && waves > 0 ? waves - 1 : waves) * pairs;
 }
 
-// Columns of a tile: 256 unless tiles of 192 overhang dW less.
-inline uint32_t choose_wgrad_cols(uint32_t k) {
+// Columns of a tile.  Narrow ones where they still leave no more than a tile for each pair: its sums are read, joined and stored by more CTAs at
+// a time, which is most of what few tiles take.  128 there; 64 where a pair's sum is short, or where many pairs share a tile either way (a
+// k-block of a narrow tile takes longer than its part of the products: A's rows are loaded for fewer columns).  us for 256, 128 and 64:
+//   tiles of 64 below a quarter of the pairs: 8192 tokens N=K=512 24.9, 22.2, 19.0; 20000 N=128 K=1024 39.6, 31.1, 28.5
+//   up to 16 k-blocks, tiles of 64 below the pairs: 333 N=1030 K=517 14.3, 12.6, 10.9; 2048 N=1024 K=512 14.7, 12.0, 11.3
+//   more k-blocks: 4096 N=K=1024 22.7, 18.5, 21.9; 4194 N=91 K=4352 33.0, 29.3, 34.2; 16384 N=K=1024 49.7, 44.2, 54.8
+//   tiles of 128 above the pairs: 300 N=K=2048 11.6, 12.4, 12.6; 2048 N=4096 K=2048 27.3, 31.0, 40.5; 4096 N=4096 K=1024 40.6, 38.2, 44.9
+// Otherwise 256, unless tiles of 192 overhang dW less.
+inline uint32_t choose_wgrad_cols(uint32_t n, uint32_t k, uint32_t groups, uint32_t blocks, uint32_t pairs) {
+    auto tiles = [&](uint32_t cols) { return static_cast<uint64_t>(ceil_div(n, kWgradRows)) * ceil_div(k, cols) * groups; };
+    if (tiles(64) <= pairs && (blocks <= 16ull * groups || 4 * tiles(64) <= pairs)) return 64;
+    if (tiles(128) <= pairs) return 128;
     return align_up(k, 192u) * 1.05 < align_up(k, 256u) ? 192 : 256;
 }
 
@@ -857,15 +867,16 @@ inline bool plan_wgrad_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t
     w.blocks = max_token_blocks(rows, groups, grouped);
     w.codes_ld_n = align_up(n, 16u);
     w.codes_ld_k = align_up(k, 16u);
-    w.cols = choose_wgrad_cols(k);
+    const uint32_t all_pairs = num_sms > 1 ? num_sms / 2 : 1;
+    w.cols = choose_wgrad_cols(n, k, groups, ceil_div(rows, 128u), all_pairs);
     const uint64_t tiles = static_cast<uint64_t>(ceil_div(n, kWgradRows)) * ceil_div(k, w.cols) * groups;
     if (tiles > 0x7fffffffull || static_cast<uint64_t>(w.blocks) * 128 > 0x7fffffffull || num_sms == 0) return false;
     w.tiles = static_cast<uint32_t>(tiles);
     // the length of all tiles (WgradSchedule) is counted in 32 bits
     if (tiles / groups * (w.blocks + static_cast<uint64_t>(groups) * kWgradMaxStoreCost) > 0xffffffffull) return false;
     // a pair per tile, or per kWgradMinCut k-blocks of one
-    const uint64_t useful = tiles * (1 + w.blocks / kWgradMinCut), pairs = num_sms > 1 ? num_sms / 2 : 1;
-    w.pairs = static_cast<uint32_t>(useful < pairs ? useful : pairs);
+    const uint64_t useful = tiles * (1 + w.blocks / kWgradMinCut);
+    w.pairs = static_cast<uint32_t>(useful < all_pairs ? useful : all_pairs);
     w.whole_tiles = choose_whole_wgrad_tiles(w.tiles, w.pairs);
     const bool shared = w.whole_tiles != w.tiles && w.blocks >= kWgradMinCut;  // tiles may be cut
     const uint64_t quads = max_token_quads(w.blocks, groups), scale_rows = quads * (ceil_div(n, 128u) + 2ull * ceil_div(k, w.cols));
@@ -881,7 +892,7 @@ inline bool plan_wgrad_workspace(uint32_t rows, uint32_t n, uint32_t k, uint32_t
     w.codes_n = take(static_cast<size_t>(w.blocks) * 128 * w.codes_ld_n);
     w.codes_k = take(static_cast<size_t>(w.blocks) * 128 * w.codes_ld_k);
     w.scales_n = take(quads * ceil_div(n, 128u) * kScaleTileBytes);
-    w.scales_k = take(quads * ceil_div(k, w.cols) * 2 * kScaleTileBytes);
+    w.scales_k = take(quads * ceil_div(k, w.cols) * 2 * kScaleTileBytes);  // two scale tiles for a tile of any width
     w.counters = take(w.num_counters * sizeof(uint32_t));
     w.partials = take(shared ? static_cast<size_t>(2) * w.pairs * kWgradRows * w.cols * sizeof(float) : 0);
     w.bytes = at;
@@ -951,7 +962,8 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
         maps.n = make_2d_tma_desc_u8_sw128(ws + w.codes_n, static_cast<uint64_t>(w.blocks) * 128, a.n, w.codes_ld_n, 128, ok);
         maps.k = make_2d_tma_desc_u8_sw128(ws + w.codes_k, static_cast<uint64_t>(w.blocks) * 128, a.k, w.codes_ld_k, 128, ok);
         maps.scales_n = make_scale_tiles_desc(ws + w.scales_n, static_cast<uint64_t>(w.quads) * ceil_div(a.n, 128u), 1, ok);
-        maps.scales_k = make_scale_tiles_desc(ws + w.scales_k, static_cast<uint64_t>(w.quads) * ceil_div(a.k, w.cols) * 2, 2, ok);
+        const uint32_t scale_tiles = ceil_div(w.cols, 128u);
+        maps.scales_k = make_scale_tiles_desc(ws + w.scales_k, static_cast<uint64_t>(w.quads) * ceil_div(a.k, w.cols) * scale_tiles, scale_tiles, ok);
         if (!ok) return kTensorMapFailed;
 
         CastTokensParams c;
@@ -1004,7 +1016,7 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
     // Old values are fetched ahead in bf16, and in fp32 where a tile has few k-blocks and its store is what takes long: us for 8, 16, 32 and 64
     // k-blocks per group (16 experts N=4096 K=2048; one N=7168 K=2048; 8 N=K=4096; one N=7168 K=2048) added in L2 350, 51.5, 585, 131, fetched
     // ahead 300, 50.1, 610, 138.  With a tile for each pair at most there is nothing to hide them behind (333 tokens N=1032 K=520 12.4, 12.8).
-    const bool ahead = a.accumulate && (a.out_bf16 || (w.tiles > w.pairs && a.groups.rows <= 16u * 128 * a.groups.num_groups));
+    const bool ahead = a.accumulate && w.cols >= 192 && (a.out_bf16 || (w.tiles > w.pairs && a.groups.rows <= 16u * 128 * a.groups.num_groups));
     auto launch = [&](auto out, auto vectors) {
         using out_t = decltype(out);
         constexpr bool kVector = decltype(vectors)::value;
@@ -1013,6 +1025,8 @@ inline int launch_fp8_wgrad(const WgradArgs& a, cudaStream_t stream) {
                 return w.cols == 192 ? launch_wgrad_products<192, out_t, true, true>(p, maps, w.pairs, stream)
                                      : launch_wgrad_products<256, out_t, true, true>(p, maps, w.pairs, stream);
         }
+        if (w.cols == 64) return launch_wgrad_products<64, out_t, kVector>(p, maps, w.pairs, stream);
+        if (w.cols == 128) return launch_wgrad_products<128, out_t, kVector>(p, maps, w.pairs, stream);
         return w.cols == 192 ? launch_wgrad_products<192, out_t, kVector>(p, maps, w.pairs, stream)
                              : launch_wgrad_products<256, out_t, kVector>(p, maps, w.pairs, stream);
     };
