@@ -189,15 +189,15 @@ struct WgradSchedule {
     uint32_t stretches, shortest, longer;  // the first `longer` stretches are one longer than `shortest`
 };
 
-// A pair of CTAs computes 256 x kCols of dW at a time (64, 128, 192 or 256: choose_wgrad_cols), each CTA 128 rows of it: per 128 tokens it loads 128 rows of A and kCols / 2 columns of
-// B, where a CTA by itself would load all kCols.  What bounds long sums is the power limit (1.28 GHz at N=28672 K=8192), so that bytes
-// moved per product count more than cycles.  Quantization and products together take 1.66 ms there; when the tiles were chosen it was 1.74
-// with pairs and 256 columns, 1.81 with 192 (whose two accumulators lie side by side, so that nothing ever waits for sums to be read),
-// 2.12 with 224, 1.95 with single CTAs of 128 x 256.
+// A pair of CTAs computes 256 x kCols of dW at a time (64, 128, 192 or 256: choose_wgrad_cols), each CTA 128 rows of it: per 128 tokens it
+// loads 128 rows of A and the box of B that holds its kCols / 2 columns, where a CTA by itself would need all kCols.  What bounds long
+// sums is the power limit (1.28 GHz at N=28672 K=8192), so that bytes moved per product count more than cycles.  Quantization and
+// products together take 1.66 ms there; when the tiles were chosen it was 1.74 with pairs and 256 columns, 1.81 with 192 (whose two
+// accumulators lie side by side, so that nothing ever waits for sums to be read), 2.12 with 224, 1.95 with single CTAs of 128 x 256.
 constexpr uint32_t kWgradRows = 256;
 // Parts of a tile that meet in L2 cost about as much as twelve k-blocks (us with the shortest tile that is cut and the shortest stretch at
-// 8 and 8, 24 and 12, 32 and 16 k-blocks: 2048 tokens N=1024 K=512 18.5, 14.8, 14.8; 3888 tokens N=K=128 16.8, 16.1, 14.9; 4096
-// tokens N=K=4000 83.6, 84.2, 78.7).
+// 16 and 8, 24 and 12, 32 and 16 k-blocks: 2048 tokens N=1024 K=512 12.9, 11.3, 11.3; 3000 tokens N=2048 K=1024 22.4, 22.5, 16.8; 4096
+// tokens N=K=1024 21.9, 18.7, 18.7; 3888 tokens N=K=128 12.8, 13.1, 13.6).
 constexpr uint32_t kWgradMinCut = 32, kWgradMinStretch = 16, kWgradMaxStoreCost = 20;
 
 // kOldItem: bytes of an element of dW whose old values are fetched ahead of the store that adds to them, or 0.  They wait in shared memory, and what
@@ -678,8 +678,8 @@ __global__ void __launch_bounds__(384, 1) __cluster_dims__(2, 1, 1)
                     loaded = ptx::mbar_test_wait(full + stage, phase);
                     if (i == 0 || kb % 4 == 0) {
                         // Three sets in turn.  The set that is written now was last used three quads ago.  If that was in this chain or the
-                        // one in front, at least five k-blocks lie in between, and the stage just filled was free: the products of six
-                        // k-blocks ago are complete.  If it was earlier, its accumulator has been read.
+                        // one in front, at least five k-blocks lie in between, and the stage just filled was free: the products of kStages,
+                        // at most six, k-blocks ago are complete.  If it was earlier, its accumulator has been read.
                         set = set == 2 ? 0 : set + 1;
 #pragma unroll
                         for (uint32_t t = 0; t < T::kScaleTiles; ++t)
